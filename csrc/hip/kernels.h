@@ -115,4 +115,21 @@ int tca_bias_relu_maxpool_launch(const void* x, const void* bias, void* y, int b
 // x: [batch][3][in_h][in_w] fp16 NCHW; wk: [64][192] fp16 (see conv_gemm.hip); y: [batch][PH][PW][64] fp16 NHWC.
 int tca_stem_conv_pool_launch(const void* x, const void* wk, const void* bias, void* y, int batch, int in_h, int in_w,
                               void* stream);
+
+// 8-bit integer rows with an fp32 scale per row (int8_rows.hip).  Strides are in elements between rows; dtype is that of
+// the floating operands.  gated: x holds 2 * width values per row, silu(first half) * second half is quantised.
+int tca_int8_quantize_launch(const void* x, void* q, void* scale, int dtype, int gated, long long rows, long long width,
+                             long long x_stride, long long q_stride, void* stream);
+// residual and sum both, or neither; sum may be x or residual
+int tca_int8_rms_norm_launch(const void* x, const void* residual, const void* weight, void* q, void* scale, void* sum,
+                             int dtype, int weight_f32, double eps, long long rows, long long width, long long x_stride,
+                             long long residual_stride, long long q_stride, long long sum_stride, void* stream);
+int tca_int8_dequantize_launch(const void* q, const void* scale, void* out, int dtype, long long rows, long long width,
+                               long long q_stride, long long out_stride, void* stream);
+// y[m][n] = round((sum_k x[m][k] w[n][k]) x_scale[m] w_scale[n] + bias[n] + residual[m][n]); k <= 131071; bias and
+// residual (null or in y's type); y may be residual (int8_linear.hip)
+int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, const void* w_scale, const void* bias,
+                           const void* residual, void* y, int dtype, long long m, long long n, long long k,
+                           long long x_stride, long long w_stride, long long residual_stride, long long y_stride,
+                           void* stream);
 }

@@ -1,0 +1,446 @@
+"""8-bit integer operators against plain references in 64 bits.
+
+The integers of a row are one well-defined answer (the nearest level of the exact quotient) and are compared for
+equality, except behind the gated activation, whose fp32 exp may move a value that lies on a border.  Tolerances count
+roundings: half a step is 2^-24 of an fp32 value, ``finfo.eps / 2`` of an output."""
+import pytest
+import torch
+
+from triton_client_amd.ops import int8
+
+pytestmark = pytest.mark.gpu
+
+F32 = 2.0 ** -24  # half a step of fp32, relative
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def _values(rows, width, dtype, seed=0, spread=1.0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, width, generator=g) * torch.exp(torch.randn(rows, 1, generator=g)) * spread
+    return x.to(dtype)
+
+
+def _levels(p):
+    """``(q, max)`` of fp32 rows on the CPU, the quotient in 64 bits (127 p is exact there, and a quotient of two fp32
+    numbers that is not a border between integers does not round to one)."""
+    top = p.abs().amax(dim=-1, keepdim=True)
+    q = torch.where(top > 0, torch.round(127 * p.double() / top.double()), 0.0)
+    return q.to(torch.int8), top
+
+
+def _int8(rows, width, seed=0, low=-127):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(low, 128, (rows, width), generator=g, dtype=torch.int8)
+
+
+WIDTHS = [1, 2, 7, 8, 9, 63, 500, 512, 513, 1000, 4095, 4096, 5000, 8192, 8200, 20001, 32768, 32769, 40000]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", WIDTHS)
+def test_quantize_is_the_nearest_level(width, dtype):
+    x = _values(5, width, dtype, seed=width)
+    q, scale = int8.quantize_int8(x.cuda())
+    ref, top = _levels(x.float())
+    assert torch.equal(q.cpu(), ref)
+    assert torch.equal(scale.cpu(), top[:, 0] / 127)  # one division, correctly rounded on both sides
+
+
+def test_quantize_special_rows():
+    inf, nan = float("inf"), float("nan")
+    top = torch.finfo(torch.float32).max
+    tiny = 2.0 ** -149
+    rows = [
+        [0.0, -0.0, 0.0, 0.0],
+        [1.0, 0.5, -0.5, 0.25],            # 63.5 is a tie: to the even 64
+        [nan, 1.0, 2.0, 3.0],
+        [1.0, inf, 2.0, 3.0],
+        [1.0, 2.0, -inf, 3.0],
+        [top, -top, top / 2, 1.0],
+        [tiny, -tiny, 0.0, tiny],          # 127 / m overflows fp32
+        [127 * tiny, 63 * tiny, -64 * tiny, tiny],
+        [1e-36, 5e-37, -3e-37, 1e-38],
+        [127.0, 0.5, -0.5, 1.5],           # ties at small levels: 0, -0, 2
+        [254.0, 125.0, 127.0, -129.0],     # 62.5, 63.5, -64.5
+    ]
+    x = torch.tensor(rows)
+    q, scale = (t.cpu() for t in int8.quantize_int8(x.cuda()))
+    finite = torch.isfinite(x).all(dim=1)
+    ref, big = _levels(x[finite])
+    assert torch.equal(q[finite], ref)
+    want = big[:, 0] / 127
+    # 127 * fp32(max / 127) of the largest fp32 value rounds to infinity: the scale one step below does not
+    want = torch.where(torch.isfinite(want * 127), want, torch.nextafter(want, torch.zeros(())))
+    assert torch.equal(scale[finite], want)
+    assert q[1].tolist() == [127, 64, -64, 32] and q[9].tolist() == [127, 0, 0, 2]
+    assert torch.isnan(scale[~finite]).all() and not q[~finite].any()
+    back = int8.dequantize_int8(q.cuda(), scale.cuda(), dtype=torch.float32).cpu()
+    assert torch.isnan(back[~finite]).all() and torch.isfinite(back[finite]).all()
+
+
+def test_quantize_every_pair_of_half_values_near_borders():
+    """All magnitudes of fp16 against maxima at which many quotients are borders or next to one."""
+    every = torch.arange(0, 0x7c00, dtype=torch.int32).to(torch.int16).view(torch.float16)
+    tops = [1.0, 127.0, 254.0, 1.9990234375, 3.96875, 6.0e-8, 65504.0, 0.0999755859375]
+    x = torch.stack([torch.where(every <= t, every, torch.tensor(t, dtype=torch.float16)) for t in tops])
+    q, _ = int8.quantize_int8(x.cuda())
+    assert torch.equal(q.cpu(), _levels(x.float())[0])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("weight_f32", [False, True])
+@pytest.mark.parametrize("width", [1, 9, 512, 1000, 4096, 5000, 8200, 32769, 40000])
+def test_norm(width, dtype, weight_f32):
+    x, r = _values(4, width, dtype, seed=1), _values(4, width, dtype, seed=2, spread=3.0)
+    w = (1 + 0.2 * _values(1, width, torch.float32, seed=3)[0]).to(torch.float32 if weight_f32 else dtype)
+    for residual in (None, r):
+        got = int8.rms_norm_int8(x.cuda(), w.cuda(), residual=None if residual is None else residual.cuda(), eps=1e-5)
+        h = x if residual is None else (x.float() + residual.float()).to(dtype)
+        if residual is not None:
+            assert torch.equal(got[2].cpu(), h)
+        q, top = _levels(h.float() * w.float())
+        assert torch.equal(got[0].cpu(), q)
+        factor = torch.rsqrt(h.double().square().mean(dim=-1, keepdim=True) + 1e-5)
+        scale = (top.double() * factor / 127)[:, 0]
+        # 64 bits until one rounding to fp32
+        assert ((got[1].cpu().double() - scale).abs() <= 1.001 * F32 * scale).all()
+
+
+def test_norm_special_rows():
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[0.0] * 4, [1.0, nan, 2.0, 3.0], [inf, 1.0, 1.0, 1.0], [3e38, -3e38, 1e38, 0.0],
+                      [2e30, 1e30, -5e29, 1.0], [1e-30, 1e-31, 0.0, 0.0], [1.0, 2.0, 3.0, 4.0]])
+    w = torch.tensor([1.0, 1.0, 0.5, 1.0])
+    q, scale = (t.cpu() for t in int8.rms_norm_int8(x.cuda(), w.cuda(), eps=1e-6))
+    bad = torch.tensor([False, True, True, False, False, False, False])
+    assert torch.isnan(scale[bad]).all() and not q[bad].any()
+    ref, top = _levels(x[~bad] * w)
+    assert torch.equal(q[~bad], ref)
+    h = x[~bad].double()  # squares of 3e38 hold in 64 bits
+    want = top[:, 0].double() / torch.sqrt(h.square().mean(dim=1) + 1e-6) / 127
+    assert ((scale[~bad].double() - want).abs() <= 1.001 * F32 * want).all()
+    # a product with the weight that leaves fp32's range counts as not finite
+    q, scale = int8.rms_norm_int8(x[3:4].cuda(), (w * 2).cuda())
+    assert torch.isnan(scale).all() and not q.any()
+
+
+@pytest.mark.parametrize("width", [1000, 40000])  # in registers, and read twice
+@pytest.mark.parametrize("which", ["x", "residual"])
+def test_norm_sum_in_place(width, which):
+    x, r = (_values(3, width, torch.bfloat16, seed=s).cuda() for s in (1, 2))
+    w = _values(1, width, torch.bfloat16, seed=3)[0].cuda()
+    want = int8.rms_norm_int8(x, w, residual=r)
+    target = x if which == "x" else r
+    got = int8.rms_norm_int8(x, w, residual=r, sum_out=target)
+    assert got[2] is target
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", [1, 7, 8, 500, 1000, 4097, 8192, 33000])
+def test_gate(width, dtype):
+    x = _values(4, 2 * width, dtype, seed=width, spread=2.0)
+    q, scale = (t.cpu() for t in int8.silu_mul_int8(x.cuda()))
+    g, u = x.double().chunk(2, dim=-1)
+    p = g / (1 + torch.exp(-g)) * u
+    top = p.abs().amax(dim=-1, keepdim=True)
+    # exp is good to one step (2 half steps); the sum, the quotient and the product round once each: 5 half steps on
+    # p and on the maximum, so 10 on a quotient of up to 127
+    assert ((q.double() - torch.where(top > 0, 127 * p / top, 0.0)).abs() <= 0.5 + 127 * 10.1 * F32).all()
+    want = (top / 127)[:, 0]
+    assert ((scale.double() - want).abs() <= 6.1 * F32 * want + 2.0 ** -149).all()
+
+
+def test_gate_extremes():
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[-100.0, 1.0, 2.0, 3.0], [-1e4, 1.0, 2.0, 3.0], [100.0, 0.0, 2.0, 3.0], [nan, 1.0, 2.0, 3.0],
+                      [1.0, 1.0, inf, 0.0], [0.0, 0.0, 5.0, 5.0]])
+    q, scale = (t.cpu() for t in int8.silu_mul_int8(x.cuda()))
+    assert q[0].tolist() == [0, 127] and q[1].tolist() == [0, 127] and q[2].tolist() == [127, 0]
+    assert torch.isnan(scale[3:5]).all() and not q[3:].any() and scale[5] == 0
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (5, 8), (2, 4097), (64, 512)])
+def test_dequantize(shape, dtype):
+    q, scale = _int8(*shape, low=-128), _values(1, shape[0], torch.float32)[0].abs()
+    got = int8.dequantize_int8(q.cuda(), scale.cuda(), dtype=dtype)
+    assert torch.equal(got.cpu(), (q.float() * scale[:, None]).to(dtype))
+
+
+def _linear_reference(x, xs, w, ws, bias, residual, dtype):
+    """The result in 64 bits, and how far the kernel may be from it."""
+    acc = x.double() @ w.double().t()  # exact: below 2^53
+    v = acc * xs.double()[:, None] * ws.double()
+    # the sum to fp32, the two scales' product and the product with it: a half step each; one more for each addition
+    slack = 3.01 * F32 * v.abs()
+    for t in (bias, residual):
+        if t is not None:
+            v = v + t.double()
+            slack = slack + 1.01 * F32 * v.abs()
+    info = torch.finfo(dtype)
+    return v, slack + info.eps / 2 * (v.abs() + slack) + info.smallest_normal * info.eps / 2
+
+
+def _linear_case(m, n, k, dtype, bias=False, residual=False, seed=0, x=None, w=None, **kw):
+    x = _int8(m, k, seed=seed + 1, low=-128) if x is None else x
+    w = _int8(n, k, seed=seed + 2, low=-128) if w is None else w
+    g = torch.Generator().manual_seed(seed)
+    xs, ws = torch.rand(m, generator=g) * 0.02 + 1e-3, torch.rand(n, generator=g) * 1e-3 + 1e-4
+    b = torch.randn(n, generator=g).to(dtype) if bias else None
+    r = torch.randn(m, n, generator=g).to(dtype) if residual else None
+    dev = [t if t is None else t.cuda() for t in (x, xs, w, ws, b, r)]
+    y = int8.linear_int8(dev[0], dev[1], dev[2], dev[3], bias=dev[4], residual=dev[5], dtype=dtype, **kw)
+    ref, slack = _linear_reference(*(t if t is None else t.cuda() for t in (x, xs, w, ws, b, r)), dtype)
+    off = (y.double() - ref).abs()
+    assert y.dtype == dtype and tuple(y.shape) == (m, n)
+    assert (off <= slack).all(), (m, n, k, float((off - slack).max()))
+    return y
+
+
+LINEAR_SHAPES = [(1, 1, 1), (1, 16, 64), (1, 4096, 4096), (2, 3, 15), (3, 17, 16), (5, 33, 17), (8, 1000, 2048),
+                 (15, 100, 127), (16, 64, 128), (17, 65, 129), (32, 128, 255), (33, 130, 256), (48, 500, 1001),
+                 (63, 63, 63), (64, 64, 640), (65, 1000, 513), (100, 257, 2000), (128, 128, 128), (129, 384, 1024),
+                 (200, 1000, 2049), (256, 256, 96), (257, 513, 4000), (300, 1000, 2048), (500, 2048, 1040),
+                 (777, 777, 777), (1024, 1024, 512), (1025, 2050, 1056)]
+
+
+@pytest.mark.parametrize("m,n,k", LINEAR_SHAPES)
+def test_linear_shapes(m, n, k):
+    _linear_case(m, n, k, torch.float16, seed=m)
+    _linear_case(m, n, k, torch.float32, bias=True, residual=True, seed=n)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("residual", [False, True])
+def test_linear_epilogues(dtype, bias, residual):
+    for m, n, k in ((7, 50, 192), (90, 203, 320), (600, 520, 400)):
+        _linear_case(m, n, k, dtype, bias=bias, residual=residual)
+
+
+@pytest.mark.parametrize("m", [1, 20, 70, 300])
+def test_linear_is_exact_at_the_largest_sums(m):
+    """128 * 128 * 131071 is the largest magnitude that int32 holds; -128 on both sides reaches it."""
+    k = int8.MAX_K
+    x = torch.full((m, k), -128, dtype=torch.int8)
+    w = torch.full((20, k), -128, dtype=torch.int8)
+    w[1] = 127
+    w[2, ::2] = 127
+    w[3, -1] = 127
+    y = int8.linear_int8(x.cuda(), torch.ones(m).cuda(), w.cuda(), torch.ones(20).cuda(), dtype=torch.float32)
+    want = (x[:1].double() @ w.double().t()).float()  # one rounding, as the kernel's
+    assert torch.equal(y.cpu(), want.expand(m, 20))
+
+
+def test_linear_selects_each_k():
+    """One-hot rows: every position of k reaches its output, in every place of a tile."""
+    k = 300
+    x = torch.eye(k, dtype=torch.int8)
+    w = _int8(70, k, seed=5)
+    ones = torch.ones
+    y = int8.linear_int8(x.cuda(), ones(k).cuda(), w.cuda(), ones(70).cuda(), dtype=torch.float32)
+    assert torch.equal(y.cpu(), w.t().float())
+
+
+@pytest.mark.parametrize("m", [4, 40, 400])
+def test_linear_rows_apart_and_unaligned(m):
+    """Column ranges of wider buffers at any alignment: neighbours are not read into the sums, nor written."""
+    n, k = 150, 200
+    for x_at, w_at, y_at in ((0, 0, 0), (1, 3, 1), (16, 32, 8), (5, 16, 3)):
+        xb, wb = _int8(m, k + 48, seed=1).cuda(), _int8(n, k + 56, seed=2).cuda()
+        x, w = xb[:, x_at:x_at + k], wb[:, w_at:w_at + k]
+        xs, ws = torch.rand(m).cuda() * 0.01, torch.rand(n).cuda() * 0.01
+        yb = torch.full((m, n + 20), 7.0, dtype=torch.float16, device="cuda")
+        rb = torch.randn(m, n + 9, device="cuda").half()
+        y = yb[:, y_at:y_at + n]
+        got = int8.linear_int8(x, xs, w, ws, residual=rb[:, 2:2 + n], out=y)
+        assert got is y
+        ref, slack = _linear_reference(x, xs, w, ws, None, rb[:, 2:2 + n], torch.float16)
+        assert ((y.double() - ref).abs() <= slack).all()
+        assert (yb[:, :y_at] == 7).all() and (yb[:, y_at + n:] == 7).all()
+
+
+def test_linear_in_place_residual_and_nan_scale():
+    x, w = _int8(70, 256).cuda(), _int8(96, 256, seed=3).cuda()
+    xs, ws = torch.rand(70).cuda(), torch.rand(96).cuda() * 1e-3
+    r = torch.randn(70, 96, device="cuda").bfloat16()
+    want = int8.linear_int8(x, xs, w, ws, residual=r, dtype=torch.bfloat16)
+    got = int8.linear_int8(x, xs, w, ws, residual=r, out=r)
+    assert got is r and torch.equal(r, want)
+    xs[3] = float("nan")
+    y = int8.linear_int8(x, xs, w, ws)
+    assert torch.isnan(y[3]).all() and torch.isfinite(y[torch.arange(70) != 3]).all()
+
+
+def test_shapes_of_any_rank_and_layout():
+    x = _values(6, 40, torch.float16).reshape(2, 3, 40)
+    q, s = int8.quantize_int8(x.cuda())
+    ref = _levels(x.float())[0]
+    assert q.shape == (2, 3, 40) and s.shape == (2, 3) and torch.equal(q.cpu(), ref)
+    q1, s1 = int8.quantize_int8(x[0, 0].cuda())
+    assert q1.shape == (40,) and s1.shape == () and torch.equal(q1.cpu(), ref[0, 0])
+    q2, s2 = int8.quantize_int8(x.cuda().transpose(0, 1))
+    assert torch.equal(q2, q.transpose(0, 1)) and torch.equal(s2, s.transpose(0, 1))
+    q3, _ = int8.quantize_int8(x.cuda().reshape(6, 40)[:, ::2])
+    assert torch.equal(q3.cpu(), _levels(x.reshape(6, 40)[:, ::2].float())[0])
+    q4, _ = int8.quantize_int8(x[0, :1].cuda().expand(5, 40))
+    assert torch.equal(q4.cpu(), ref[0, :1].expand(5, 40))
+    w = _int8(12, 40, seed=9).cuda()
+    ws = torch.rand(12).cuda()
+    y = int8.linear_int8(q, s, w, ws)
+    assert y.shape == (2, 3, 12)
+    assert torch.equal(int8.linear_int8(q1, s1, w, ws), y[0, 0])
+    assert torch.equal(int8.linear_int8(q.transpose(0, 1), s.t(), w, ws), y.transpose(0, 1))
+
+
+def test_empty_batches():
+    for dtype in TYPES:
+        x = torch.empty(0, 64, dtype=dtype, device="cuda")
+        q, s = int8.quantize_int8(x)
+        assert q.shape == (0, 64) and s.shape == (0,)
+        assert int8.dequantize_int8(q, s, dtype=dtype).shape == (0, 64)
+        assert int8.rms_norm_int8(x, torch.ones(64, dtype=dtype, device="cuda"), residual=x)[2].shape == (0, 64)
+        assert int8.silu_mul_int8(x)[0].shape == (0, 32)
+        w, ws = _int8(5, 64).cuda(), torch.ones(5).cuda()
+        assert int8.linear_int8(q, s, w, ws).shape == (0, 5)
+        assert int8.linear_int8(_int8(3, 64).cuda(), torch.ones(3).cuda(), w[:0], ws[:0]).shape == (3, 0)
+
+
+def test_row_operators_into_slices():
+    """Destinations inside larger buffers: what lies around them stays."""
+    x = _values(9, 100, torch.bfloat16).cuda()
+    w = torch.ones(100, dtype=torch.bfloat16, device="cuda")
+    qb = torch.full((9, 130), 55, dtype=torch.int8, device="cuda")
+    sb = torch.full((11,), 5.0, device="cuda")
+    hb = torch.full((9, 120), 5.0, dtype=torch.bfloat16, device="cuda")
+    want = int8.rms_norm_int8(x, w, residual=x)
+    int8.rms_norm_int8(x, w, residual=x, out=qb[:, 3:103], scale=sb[1:10], sum_out=hb[:, 7:107])
+    assert torch.equal(qb[:, 3:103], want[0]) and torch.equal(sb[1:10], want[1]) and torch.equal(hb[:, 7:107], want[2])
+    assert (qb[:, :3] == 55).all() and (qb[:, 103:] == 55).all()
+    assert sb[0] == 5 and sb[10] == 5 and (hb[:, :7] == 5).all() and (hb[:, 107:] == 5).all()
+    yb = torch.full((9, 111), 5.0, device="cuda")
+    int8.dequantize_int8(qb[:, 3:103], sb[1:10], out=yb[:, 1:101])
+    assert torch.equal(yb[:, 1:101], want[0].float() * want[1][:, None])
+    assert (yb[:, :1] == 5).all() and (yb[:, 101:] == 5).all()
+    # column ranges of one buffer lie apart
+    both = torch.zeros(9, 200, dtype=torch.bfloat16, device="cuda")
+    both[:, :100] = x
+    int8.rms_norm_int8(both[:, :100], w, residual=x, sum_out=both[:, 100:])
+    assert torch.equal(both[:, 100:], want[2]) and torch.equal(both[:, :100], x)
+
+
+def _block(x, h, norm, w1, s1, w2, s2):
+    q, s, h = int8.rms_norm_int8(x, norm, residual=h)
+    y = int8.linear_int8(q, s, w1, s1, dtype=x.dtype)
+    q, s = int8.silu_mul_int8(y)
+    return int8.linear_int8(q, s, w2, s2, residual=h, dtype=x.dtype)
+
+
+def _block_operands(d, f, dtype):
+    w1, w2 = _values(2 * f, d, torch.float32, 1, d ** -0.5), _values(d, f, torch.float32, 2, f ** -0.5)
+    norm = (1 + 0.1 * _values(1, d, torch.float32, 3)[0]).to(dtype)
+    return norm.cuda(), *int8.quantize_int8(w1.cuda()), *int8.quantize_int8(w2.cuda())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("tokens", [1, 5, 64, 333])
+def test_block_together(tokens, dtype):
+    """Norm, product, gated activation, product and residual, as a model runs them, each step against its formula on
+    what the step before handed over."""
+    d, f = 320, 456
+    ops = _block_operands(d, f, dtype)
+    x, h0 = _values(tokens, d, dtype, 4).cuda(), _values(tokens, d, dtype, 5).cuda()
+    out = _block(x, h0, *ops)
+    norm, w1, s1, w2, s2 = ops
+    q, s, h = int8.rms_norm_int8(x, norm, residual=h0)
+    assert torch.equal(q.cpu(), _levels((h.float() * norm.float()).cpu())[0])
+    y = int8.linear_int8(q, s, w1, s1, dtype=dtype)
+    ref, slack = _linear_reference(q, s, w1, s1, None, None, dtype)
+    assert ((y.double() - ref).abs() <= slack).all()
+    q, s = int8.silu_mul_int8(y)
+    g, u = y.double().chunk(2, dim=-1)
+    p = g / (1 + torch.exp(-g)) * u
+    t = 127 * p / p.abs().amax(dim=-1, keepdim=True)
+    assert ((q.double() - t).abs() <= 0.5 + 127 * 10.1 * F32).all()
+    ref, slack = _linear_reference(q, s, w2, s2, None, h, dtype)
+    assert ((out.double() - ref).abs() <= slack).all()
+
+
+def test_block_in_a_graph_and_on_other_streams():
+    """Captured and replayed with new inputs, eager work between; two streams at once; results equal the eager ones."""
+    ops = _block_operands(256, 384, torch.bfloat16)
+    xs = [_values(33, 256, torch.bfloat16, s).cuda() for s in range(4)]
+    hs = [_values(33, 256, torch.bfloat16, 10 + s).cuda() for s in range(4)]
+    want = [_block(x, h, *ops) for x, h in zip(xs, hs)]
+    graphs = []
+    for _ in range(2):  # two graphs that live side by side
+        x_in, h_in = xs[0].clone(), hs[0].clone()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _block(x_in, h_in, *ops)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _block(x_in, h_in, *ops)
+        graphs.append((graph, x_in, h_in, out))
+    for turn in range(4):
+        for i, (graph, x_in, h_in, out) in enumerate(graphs):
+            k = (turn + i) % 4
+            x_in.copy_(xs[k])
+            h_in.copy_(hs[k])
+            graph.replay()
+            _block(xs[0], hs[0], *ops)
+            assert torch.equal(out, want[k])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for turn in range(6):
+        with torch.cuda.stream(streams[turn % 2]):
+            got.append(_block(xs[turn % 4], hs[turn % 4], *ops))
+    torch.cuda.synchronize()
+    for turn in range(6):
+        assert torch.equal(got[turn], want[turn % 4])
+    # the two graphs at the same time
+    for i, (graph, x_in, h_in, _) in enumerate(graphs):
+        x_in.copy_(xs[i])
+        h_in.copy_(hs[i])
+    torch.cuda.synchronize()
+    for i, (graph, *_rest) in enumerate(graphs):
+        with torch.cuda.stream(streams[i]):
+            graph.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(graphs[i][3], want[i])
+
+
+def test_offsets_beyond_32_bits():
+    rows, width = (1 << 31) // 4096 + 3, 4096  # more than 2^31 values
+    x = torch.zeros(rows, width, dtype=torch.float16, device="cuda")
+    tail = _values(4, width, torch.float16).cuda()
+    x[-4:] = tail
+    x[0] = tail[0]
+    q, s = int8.quantize_int8(x)
+    wq, ws = int8.quantize_int8(tail)
+    assert torch.equal(q[-4:], wq) and torch.equal(s[-4:], ws) and torch.equal(q[0], wq[0]) and not q[1:-4].any()
+    back = int8.dequantize_int8(q, s)
+    assert torch.equal(back[-4:], int8.dequantize_int8(wq, ws))
+    norm = torch.ones(width, dtype=torch.float16, device="cuda")
+    got = int8.rms_norm_int8(x, norm, residual=back, sum_out=back)
+    want = int8.rms_norm_int8(tail, norm, residual=int8.dequantize_int8(wq, ws))
+    for a, b in zip(got, want):
+        assert torch.equal(a[-4:], b)
+    del x, back, got
+    w, sw = _int8(24, width).cuda(), torch.rand(24).cuda()
+    y = int8.linear_int8(q, s, w, sw, dtype=torch.float32)
+    assert torch.equal(y[-4:], int8.linear_int8(wq, ws, w, sw, dtype=torch.float32)) and not y[1:-4].any()
+    # as the weight, and with an output of more than 2^31 values
+    y = int8.linear_int8(w, sw, q, s, dtype=torch.float32)
+    assert torch.equal(y[:, -4:], int8.linear_int8(w, sw, wq, ws, dtype=torch.float32))
+    del y
+    a, sa = _int8(40000, 16, seed=1).cuda(), torch.rand(40000).cuda()
+    b, sb = _int8(60000, 16, seed=2).cuda(), torch.rand(60000).cuda()
+    y = int8.linear_int8(a, sa, b, sb)
+    assert torch.equal(y[-300:], int8.linear_int8(a[-300:].clone(), sa[-300:], b, sb))

@@ -6,6 +6,8 @@
 ``codec``         BYTES tensor pack / index / gather, BF16 <-> FP32
 ``classification`` top-k and ``"value:index:label"`` payload formatting
 ``head``          MFMA fully connected classification head (fp16)
+``int8``          8-bit integer operators of language models: rows, norm, gated
+                  activation, matrix product
 ================  ==========================================================
 
 All kernels live in ``csrc/hip`` and are compiled into ``libtca_hip.so`` for

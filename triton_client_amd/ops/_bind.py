@@ -1,6 +1,6 @@
 """ctypes prototypes of ``libtca_hip.so`` (hipshm + CDNA4 kernel launchers)."""
 
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_longlong, c_uint8, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_longlong, c_uint8, c_uint32, c_uint64, c_void_p
 
 
 class PreprocImage(Structure):
@@ -142,6 +142,20 @@ def install(lib):
     lib.tca_bias_relu_maxpool_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]
     lib.tca_stem_conv_pool_launch.restype = c_int
     lib.tca_stem_conv_pool_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]
+    lib.tca_int8_quantize_launch.restype = c_int
+    lib.tca_int8_quantize_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_int, c_longlong, c_longlong,
+                                             c_longlong, c_longlong, c_void_p]
+    lib.tca_int8_rms_norm_launch.restype = c_int
+    lib.tca_int8_rms_norm_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+                                             c_double, c_longlong, c_longlong, c_longlong, c_longlong, c_longlong,
+                                             c_longlong, c_void_p]
+    lib.tca_int8_dequantize_launch.restype = c_int
+    lib.tca_int8_dequantize_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_int, c_longlong, c_longlong, c_longlong,
+                                               c_longlong, c_void_p]
+    lib.tca_int8_linear_launch.restype = c_int
+    lib.tca_int8_linear_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                           c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_longlong,
+                                           c_longlong, c_void_p]
     install_rt(lib)
 
 

@@ -1,0 +1,353 @@
+"""8-bit integer operators for serving language models (inference).
+
+``quantize_int8``    rows to 8-bit integers with one fp32 scale per row
+``dequantize_int8``  the values such rows stand for
+``rms_norm_int8``    root-mean-square norm with the residual's addition, straight to 8-bit rows
+``silu_mul_int8``    the gated activation of an MLP, straight to 8-bit rows
+``linear_int8``      matrix product of 8-bit rows with 8-bit weights, a scale per token and per output channel,
+                     bias and residual in the epilogue
+
+The kernels are ``csrc/hip/int8_rows.hip`` and ``csrc/hip/int8_linear.hip``.  A block of a model runs them back to back,
+activations crossing memory in 8 bits between the products::
+
+    w1, s1 = quantize_int8(gate_up_weight)                      # once, [2 * F, D]
+    w2, s2 = quantize_int8(down_weight)                         # once, [D, F]
+    q, s, h = rms_norm_int8(x, norm_weight, residual=h)
+    y = linear_int8(q, s, w1, s1, dtype=torch.bfloat16)         # [tokens, 2 * F]
+    q, s = silu_mul_int8(y)
+    h = linear_int8(q, s, w2, s2, residual=h, dtype=torch.bfloat16)
+
+Rows are everything but the last axis.  Inputs are torch CUDA tensors of fp16, bf16 or fp32 (integers: int8); rows may
+lie apart (a 2-D view with a row stride), other layouts are copied first.  Work is enqueued on the current torch stream
+of the tensors' device and nothing waits for it; results may be captured into graphs.  The integers have no gradient:
+operands that require one are refused while gradients are recorded.
+
+A row with a value that is not finite gets integers of 0 and a scale of NaN, so that whatever is computed from it is NaN
+instead of a number.  The reference has no model code (its models run in the server it talks to, e.g.
+``src/python/examples/image_client.py:59-150`` only inspects metadata); this is the serving side of that contract.
+"""
+
+from __future__ import annotations
+
+from ._device import check, lib
+
+# 128 * 128 * k has to stay below 2^31
+MAX_K = 131071
+MAX_WIDTH = 1 << 29
+
+_TYPE_CODE = None
+
+
+def _codes():
+    import torch
+
+    global _TYPE_CODE
+    if _TYPE_CODE is None:
+        _TYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    return _TYPE_CODE
+
+
+def _float_code(t, name):
+    code = _codes().get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be an fp16, bf16 or fp32 tensor")
+    return code
+
+
+def _output_code(dtype):
+    code = _codes().get(dtype)
+    if code is None:
+        raise TypeError("dtype must be torch.float16, torch.bfloat16 or torch.float32")
+    return code
+
+
+def _refuse_gradients(*operands):
+    import torch
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
+        raise ValueError("8-bit operators have no gradient: detach the operands or call under torch.no_grad()")
+
+
+def _same_device(first, *others):
+    """The common CUDA device of the operands."""
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError("the operands must be CUDA tensors")
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError("the operands must be on one device")
+    return device
+
+
+def _rows(t):
+    """``(tensor, row stride)`` of an input: as it is where the values of a row lie side by side, else a copy."""
+    if t.is_contiguous():
+        return t, t.shape[-1]
+    if t.dim() == 2 and t.stride(1) == 1:
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[-1]
+
+
+def _out_rows(out, shape, dtype, device, name):
+    """Row stride of a caller's destination."""
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != device:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)} on {device}")
+    if out.requires_grad:
+        raise ValueError(f"{name} must not require a gradient")
+    if out.is_contiguous():
+        return out.shape[-1] if out.dim() else 1
+    if out.dim() == 2 and out.stride(1) == 1 and out.stride(0) >= out.shape[1]:
+        return out.stride(0)
+    raise ValueError(f"{name} must be contiguous, or 2-D with contiguous rows that do not overlap")
+
+
+def _extent(t):
+    """``(first byte, one past the last, bytes between rows, bytes of a row)`` of a tensor with contiguous rows."""
+    first, size = t.data_ptr(), t.element_size()
+    if t.is_contiguous():
+        return first, first + t.numel() * size, 0, 0
+    stride, row = t.stride(0) * size, t.shape[1] * size
+    return first, first + (t.shape[0] - 1) * stride + row, stride, row
+
+
+def _overlap(a, b):
+    if not a.numel() or not b.numel():
+        return False
+    a0, a1, a_stride, a_row = _extent(a)
+    b0, b1, b_stride, b_row = _extent(b)
+    if a0 >= b1 or b0 >= a1:
+        return False
+    if a_stride == b_stride and a_stride:  # column ranges of one buffer
+        apart = (a0 - b0) % a_stride
+        return apart < b_row or apart + a_row > a_stride
+    return True
+
+
+def _check_apart(outputs, inputs):
+    """Destinations ``(name, tensor or None, inputs that it may be)`` lie apart from the inputs and each other."""
+    given = [o for o in outputs if o[1] is not None]
+    for i, (name, out, may_be) in enumerate(given):
+        for t in inputs:
+            # an input that IS the destination: every value is read by the thread that writes it, before it does
+            if t is not None and _overlap(out, t) and not (any(t is m for m in may_be)
+                                                           and out.data_ptr() == t.data_ptr()
+                                                           and out.stride() == t.stride()):
+                raise ValueError(f"{name} overlaps an input")
+        for other, t, _ in given[:i]:
+            if _overlap(out, t):
+                raise ValueError(f"{name} overlaps {other}")
+
+
+def _launch(what, device, *args):
+    import torch
+
+    fn = getattr(lib(), what)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    check(rc, what)
+
+
+def _check_rows(x):
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"x must have a last axis of 1 to {MAX_WIDTH} values")
+
+
+def _row_outputs(shape, device, out, scale):
+    """``(q, q stride, scale)``: the destinations given, or new ones."""
+    import torch
+
+    if out is None:
+        out, stride = torch.empty(shape, dtype=torch.int8, device=device), shape[-1]
+    else:
+        stride = _out_rows(out, shape, torch.int8, device, "out")
+    if scale is None:
+        scale = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+    else:
+        _check_scale_out(scale, shape[:-1], device)
+    return out, stride, scale
+
+
+def _check_scale_out(scale, shape, device):
+    import torch
+
+    if (scale.dtype != torch.float32 or tuple(scale.shape) != tuple(shape) or scale.device != device
+            or not scale.is_contiguous() or scale.requires_grad):
+        raise ValueError(f"scale must be a contiguous fp32 tensor of shape {list(shape)} on {device}")
+
+
+def _quantize(x, width, gated, out, scale):
+    code = _float_code(x, "x")
+    _refuse_gradients(x)
+    device = _same_device(x, out, scale)
+    x, x_stride = _rows(x)
+    q, q_stride, s = _row_outputs((*x.shape[:-1], width), device, out, scale)
+    if out is not None or scale is not None:
+        _check_apart((("out", out, ()), ("scale", scale, ())), (x,))
+    rows = s.numel()
+    if rows:
+        _launch("tca_int8_quantize_launch", device, x.data_ptr(), q.data_ptr(), s.data_ptr(), code, gated, rows, width,
+                x_stride, q_stride)
+    return q, s
+
+
+def quantize_int8(x, out=None, scale=None):
+    """``(q int8 [..., K], scale fp32 [...])`` of ``x [..., K]``: with ``m`` the largest magnitude of a row, ``q`` is the
+    integer nearest to ``127 x / m`` (ties to even, decided exactly) and ``scale = m / 127`` (one step less where
+    ``127 * scale`` would leave fp32's range).  A row of zeros has the scale 0.  ``out`` and ``scale`` may be destinations of the results' shapes."""
+    _check_rows(x)
+    return _quantize(x, x.shape[-1], 0, out, scale)
+
+
+def silu_mul_int8(x, out=None, scale=None):
+    """8-bit rows ``(q [..., K], scale [...])``, as of :func:`quantize_int8`, of ``silu(gate) * up`` for
+    ``x [..., 2 K]`` with the gate in the first half of the last axis and the other factor in the second.  The product
+    is taken in fp32."""
+    _check_rows(x)
+    if x.shape[-1] % 2:
+        raise ValueError("the last axis of x must hold two halves of equal size")
+    return _quantize(x, x.shape[-1] // 2, 1, out, scale)
+
+
+def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_out=None):
+    """8-bit rows of ``h / sqrt(mean(h^2) + eps) * weight``: ``(q, scale)`` for ``h = x``, or ``(q, scale, h)`` for
+    ``h = x + residual``.
+
+    x         ``[..., K]``
+    weight    ``[K]``, contiguous, of x's type or fp32
+    residual  of x's shape and type, or None.  The sum is rounded to x's type, and the rounded sum is what is
+              normalised and returned: what the next block reads is what this one saw
+    sum_out   destination of the sum; may be ``x`` or ``residual`` itself
+
+    ``q`` is the integer nearest to ``127 h weight / max|h weight|`` (ties to even, decided exactly): the norm's factor
+    cancels and only enters the scale.  Sums of squares are held in 64 bits."""
+    import torch
+
+    code = _float_code(x, "x")
+    _check_rows(x)
+    width = x.shape[-1]
+    weight_f32 = weight.dtype == torch.float32
+    if not weight_f32 and weight.dtype != x.dtype:
+        raise TypeError("weight must have x's type or be fp32")
+    if tuple(weight.shape) != (width,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous vector of {width} values")
+    eps = float(eps)
+    if not 0.0 < eps < float("inf"):
+        raise ValueError("eps must be a positive number")
+    if residual is None:
+        if sum_out is not None:
+            raise ValueError("sum_out needs a residual")
+    elif residual.dtype != x.dtype or residual.shape != x.shape:
+        raise ValueError("residual must have x's type and shape")
+    _refuse_gradients(x, weight, residual)
+    device = _same_device(x, weight, residual, out, scale, sum_out)
+    shape = x.shape
+    x, x_stride = _rows(x)
+    q, q_stride, s = _row_outputs(tuple(shape), device, out, scale)
+    summed, r_ptr, sum_ptr, r_stride, sum_stride = None, None, None, 0, 0
+    if residual is not None:
+        residual, r_stride = _rows(residual)
+        if sum_out is None:
+            summed, sum_stride = torch.empty(shape, dtype=x.dtype, device=device), width
+        else:
+            summed, sum_stride = sum_out, _out_rows(sum_out, shape, x.dtype, device, "sum_out")
+        r_ptr, sum_ptr = residual.data_ptr(), summed.data_ptr()
+    if out is not None or scale is not None or sum_out is not None:
+        _check_apart((("out", out, ()), ("scale", scale, ()), ("sum_out", sum_out, (x, residual))),
+                     (x, weight, residual))
+    rows = s.numel()
+    if rows:
+        _launch("tca_int8_rms_norm_launch", device, x.data_ptr(), r_ptr, weight.data_ptr(), q.data_ptr(), s.data_ptr(),
+                sum_ptr, code, weight_f32, eps, rows, width, x_stride, r_stride, q_stride, sum_stride)
+    return (q, s) if residual is None else (q, s, summed)
+
+
+def _check_quantized(q, scale, name):
+    import torch
+
+    if q.dtype != torch.int8:
+        raise TypeError(f"{name} must be an int8 tensor")
+    if scale.dtype != torch.float32:
+        raise TypeError(f"{name}_scale must be an fp32 tensor" if name != "q" else "scale must be an fp32 tensor")
+    if q.dim() < 1 or scale.shape != q.shape[:-1]:
+        raise ValueError(f"{name} [..., K] needs a scale for each row, of shape [...]")
+
+
+def dequantize_int8(q, scale, dtype=None, out=None):
+    """``q * scale`` of 8-bit rows ``q [..., K]`` with ``scale [...]``, in ``dtype`` (default fp16, or out's)."""
+    import torch
+
+    _check_quantized(q, scale, "q")
+    if not 1 <= q.shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"q must have a last axis of 1 to {MAX_WIDTH} values")
+    if dtype is None:
+        dtype = torch.float16 if out is None else out.dtype
+    code = _output_code(dtype)
+    _refuse_gradients(scale)
+    device = _same_device(q, scale, out)
+    shape = q.shape
+    q, q_stride = _rows(q)
+    scale = scale.contiguous()
+    if out is None:
+        out, out_stride = torch.empty(shape, dtype=dtype, device=device), shape[-1]
+    else:
+        out_stride = _out_rows(out, shape, dtype, device, "out")
+        _check_apart((("out", out, ()),), (q, scale))
+    rows = scale.numel()
+    if rows:
+        _launch("tca_int8_dequantize_launch", device, q.data_ptr(), scale.data_ptr(), out.data_ptr(), code, rows,
+                shape[-1], q_stride, out_stride)
+    return out
+
+
+def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtype=None, out=None):
+    """``(x weight^T) * x_scale * weight_scale + bias (+ residual)`` in ``dtype`` (default fp16, or out's).
+
+    x, x_scale            8-bit rows ``[..., K]`` with a scale per token ``[...]``
+    weight, weight_scale  8-bit rows ``[N, K]`` with a scale per output channel ``[N]``
+    bias                  ``[N]`` in ``dtype``, contiguous, or None
+    residual              ``[..., N]`` in ``dtype``, or None; ``out`` may be the residual itself
+
+    Sums are int32 and exact for K up to 131071; scales, bias and residual are applied in fp32 and the result is rounded
+    once.  Rows that start at multiples of 16 bytes (K, or the row stride, a multiple of 16) are read fastest."""
+    import torch
+
+    _check_quantized(x, x_scale, "x")
+    _check_quantized(weight, weight_scale, "weight")
+    if weight.dim() != 2:
+        raise ValueError("weight must be an [N, K] matrix")
+    n, k = weight.shape
+    if x.shape[-1] != k:
+        raise ValueError(f"x has rows of {x.shape[-1]} integers, weight of {k}")
+    if not 1 <= k <= MAX_K:
+        raise ValueError(f"K must be 1 to {MAX_K}: the int32 sums hold no more")
+    if dtype is None:
+        dtype = torch.float16 if out is None else out.dtype
+    code = _output_code(dtype)
+    shape = (*x.shape[:-1], n)
+    if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous {dtype} vector of {n} values")
+    if residual is not None and (residual.dtype != dtype or tuple(residual.shape) != shape):
+        raise ValueError(f"residual must be a {dtype} tensor of shape {list(shape)}")
+    _refuse_gradients(x_scale, weight_scale, bias, residual)
+    device = _same_device(x, x_scale, weight, weight_scale, bias, residual, out)
+    x, x_stride = _rows(x)
+    weight, w_stride = _rows(weight)
+    x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
+    r_ptr, r_stride = None, 0
+    if residual is not None:
+        residual, r_stride = _rows(residual)
+        r_ptr = residual.data_ptr()
+    if out is None:
+        out, out_stride = torch.empty(shape, dtype=dtype, device=device), n
+    else:
+        out_stride = _out_rows(out, shape, dtype, device, "out")
+        _check_apart((("out", out, (residual,)),), (x, x_scale, weight, weight_scale, bias, residual))
+    tokens = x_scale.numel()
+    if tokens and n:
+        _launch("tca_int8_linear_launch", device, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
+                weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), r_ptr, out.data_ptr(), code, tokens,
+                n, k, x_stride, w_stride, r_stride, out_stride)
+    return out
