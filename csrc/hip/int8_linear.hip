@@ -13,9 +13,16 @@
 //
 // SplitKernel  the waves of a block share the k axis of one small output tile: every wave multiplies its own k steps of
 //              128 straight from memory to registers, the partial sums meet in LDS.
+// TileKernel   large products: 256 x 256 (or 128 x 128) outputs per block of four waves, operands through a ring of LDS
+//              stages filled by DMA.  8192 x 8192 x 8192 to bf16: 408 us (2.69 POP/s), 462 us with a residual.  What
+//              bounds it is the card's power: on zeros, where nothing toggles, the same call takes 303 us.  One wave per
+//              SIMD with 128 x 128 outputs reads the fewest bytes from LDS per product and wins over two waves with
+//              128 x 64 (420 us); products of 16 x 16 x 64 touch the accumulators half as often per operation as those of
+//              32 x 32 x 32 and win although they issue twice as often (443 against 476 us at the same stage of tuning).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "kernels.h"
 
@@ -35,6 +42,7 @@ struct LinearArgs {
   long long x_stride, w_stride, residual_stride, y_stride;
   int k;
   int dtype;
+  int vector_rows;  // every eighth output starts at a multiple of 16 bytes, in y and the residual, and n % 8 == 0
 };
 
 __device__ __forceinline__ float Load(const void* p, long long at, int dtype) {
@@ -149,6 +157,371 @@ __global__ __launch_bounds__(64 * kWaves) void SplitKernel(LinearArgs a, long lo
   }
 }
 
+// ---- Epilogue of a tile: results leave straight from the accumulators ----------------------------------------------
+
+struct Bf16 {
+  unsigned short bits;
+};
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+__device__ __forceinline__ float ToFloat(_Float16 v) { return static_cast<float>(v); }
+__device__ __forceinline__ float ToFloat(Bf16 v) { return __uint_as_float(static_cast<unsigned>(v.bits) << 16); }
+template <typename T> __device__ __forceinline__ T FromFloat(float v);
+template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
+template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) { return static_cast<_Float16>(v); }
+template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
+  return Bf16{__builtin_bit_cast(unsigned short, static_cast<__bf16>(v))};
+}
+
+// Eight consecutive values as they lie in memory.  kVector: at a multiple of 16 bytes, all inside or all outside a
+// descriptor's range; else one by one, value i at offset + i values.
+template <typename T>
+struct Eight {
+  static constexpr int kWords = 2 * sizeof(T);
+  unsigned raw[kWords];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i]);
+    else return ToFloat(__builtin_bit_cast(T, static_cast<unsigned short>(raw[i / 2] >> (16 * (i & 1)))));
+  }
+};
+
+using uint4v = __attribute__((ext_vector_type(4))) unsigned;
+
+// An offset behind every descriptor's end, also with a row's offset added: the DMA writes zeros for it, loads give zeros,
+// stores are dropped.  The host keeps the rows of a tile below 2^30 bytes.
+constexpr unsigned kOutside = 0x80000000u;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t Descriptor(const void* p, long long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(p ? bytes : 0), 0x00020000);
+}
+
+// `inside` of the eight lie in the row: all or none of them with kVector
+template <typename T, bool kVector>
+__device__ __forceinline__ Eight<T> LoadEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int inside) {
+  Eight<T> v;
+  auto at = [&](int i) { return static_cast<int>(i < inside ? offset + i * sizeof(T) : kOutside); };
+  if constexpr (kVector) {
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
+      const uint4v part = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(inside > 0 ? offset + 16 * i : kOutside), 0, 0);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v.raw[4 * i + c] = part[c];
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v.raw[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, at(i), 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned low = static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at(2 * i), 0, 0));
+      const unsigned high = static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at(2 * i + 1), 0, 0));
+      v.raw[i] = low | high << 16;
+    }
+  }
+  return v;
+}
+
+template <typename T, bool kVector>
+__device__ __forceinline__ void StoreEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int inside, const float (&v)[8]) {
+  T t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = FromFloat<T>(v[i]);
+  if constexpr (kVector) {
+    uint4v raw[sizeof(t) / 16];
+    __builtin_memcpy(raw, t, sizeof(t));
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(t) / 16); ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(raw[i], rsrc, static_cast<int>(inside > 0 ? offset + 16 * i : kOutside), 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = static_cast<int>(i < inside ? offset + i * sizeof(T) : kOutside);
+      if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t[i]), rsrc, at, 0, 0);
+      else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, t[i]), rsrc, at, 0, 0);
+    }
+  }
+}
+
+// ---- TileKernel ---------------------------------------------------------------------------------------------------
+
+using lds_ptr_t = __attribute__((address_space(3))) void*;
+
+constexpr int kTileK = 64;  // k per stage: an LDS row of an operand is 64 bytes, one MFMA deep
+
+// Wave-wide copy global -> LDS, 16 bytes per lane, to lds + 16 * lane
+__device__ __forceinline__ void DmaToLds(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int8_t* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, reinterpret_cast<lds_ptr_t>(reinterpret_cast<uintptr_t>(lds)), 16,
+                                           static_cast<int>(offset), 0, 0, 0);
+}
+
+// The tiles of a block: each of the 8 XCDs (consecutive blocks go round them) has a contiguous run of tiles, ordered in
+// bands of kBand tile rows, so that the tiles an XCD works on at a time share operands in its L2; its blocks take them
+// in turn.
+constexpr unsigned kBand = 8;
+
+struct Tiles {
+  unsigned rows, columns, run;  // of the whole product; tiles per XCD
+};
+
+struct TileCursor {
+  unsigned at;  // position in the XCD's run
+  long long m0, n0;
+  int rows, columns;  // inside the matrix; 0 past the last tile
+
+  template <int BM, int BN>
+  __device__ __forceinline__ void Place(const LinearArgs& a, const Tiles& t) {
+    const unsigned tile = (blockIdx.x & 7) * t.run + at;
+    if (at >= t.run || tile >= t.rows * t.columns) {
+      m0 = n0 = rows = columns = 0;
+      return;
+    }
+    const unsigned band = tile / (kBand * t.columns);
+    const unsigned in_band = tile - band * kBand * t.columns;
+    const unsigned high = min(kBand, t.rows - band * kBand);
+    const unsigned column = in_band / high;
+    m0 = static_cast<long long>(band * kBand + in_band - column * high) * BM;
+    n0 = static_cast<long long>(column) * BN;
+    rows = static_cast<int>(a.m - m0 < BM ? a.m - m0 : BM);
+    columns = static_cast<int>(a.n - n0 < BN ? a.n - n0 : BN);
+  }
+};
+
+// acc += w x with the accumulator pinned to the accumulation registers: given the choice, the compiler spreads the
+// 256 accumulators of a wave over both register files and copies a third of them back and forth in every step
+__device__ __forceinline__ void Mfma(int4v w, int4v x, int4v& acc) {
+  asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(acc) : "v"(w), "v"(x));
+}
+
+// The compiler does not see matrix instructions inside asm: what it needs between them and ordinary instructions that
+// touch the accumulators (16 cycles of the instruction and its write) stands here.
+__device__ __forceinline__ void SettleAccumulators() { asm volatile("s_nop 15\n\ts_nop 7"); }
+__device__ __forceinline__ void Pin(int4v& acc) { asm volatile("" : "+a"(acc)); }  // ordered with the other asm
+
+template <int kFirst, int kLast, typename F>
+__device__ __forceinline__ void Unrolled(F&& f) {
+  if constexpr (kFirst < kLast) {
+    f(std::integral_constant<int, kFirst>{});
+    Unrolled<kFirst + 1, kLast>(f);
+  }
+}
+
+// 0, 2, 3, 1 for the low two bits 0, 1, 2, 3
+__device__ __forceinline__ int Turn(int v) { return ((v ^ (v >> 1)) & 1) * 2 + ((v >> 1) & 1); }
+
+// Epilogue of a wave, 16 tokens at a time: the accumulators go through LDS (the wave's own part, so no barrier), after
+// which a lane holds eight consecutive outputs of a token and the lanes of a token cover whole cache lines.
+//
+// Without a residual kResidual may still be set: a descriptor of nothing gives zeros, as for a bias that is not there.
+template <typename T, bool kVector, bool kResidual, int kMT, int kNT>
+__device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor& tile, int m, int n, int8_t* lds, int4v (&acc)[kMT][kNT]) {
+  constexpr int kSize = sizeof(T);
+  constexpr int kLanes = kNT * 2;               // lanes of a token
+  constexpr int kRows = 64 / kLanes;            // tokens of one access
+  constexpr int kTurns = 16 / kRows;            // accesses for 16 tokens
+  constexpr int kTurnMask = kNT * 4 < 16 ? kNT * 4 - 1 : 15;
+  constexpr int kHeld = !kVector ? 1 : kSize == 2 ? 4 : 2;  // steps of 16 tokens whose residual is requested at once
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));  // addresses are computed here for every tile: kept from tile to tile they would spill
+  const int row = m + lane / kLanes, column = n + lane % kLanes * 8;
+  const int inside = tile.columns - column;
+  const auto sx_rsrc = Descriptor(a.x_scale + tile.m0, tile.rows * 4ll);
+  const auto sw_rsrc = Descriptor(a.w_scale + tile.n0, tile.columns * 4ll);
+  const auto bias_rsrc = Descriptor(a.bias ? static_cast<const T*>(a.bias) + tile.n0 : nullptr, tile.columns * kSize);
+  const auto res_rsrc = Descriptor(a.residual ? static_cast<const T*>(a.residual) + tile.m0 * a.residual_stride + tile.n0 : nullptr,
+                                   ((tile.rows - 1) * a.residual_stride + tile.columns) * kSize);
+  // rows past the end start behind the last byte of the last one
+  const auto y_rsrc = Descriptor(static_cast<T*>(a.y) + tile.m0 * a.y_stride + tile.n0,
+                                 ((tile.rows - 1) * a.y_stride + tile.columns) * kSize);
+  const unsigned y_pitch = static_cast<unsigned>(a.y_stride) * kSize, res_pitch = static_cast<unsigned>(a.residual_stride) * kSize;
+  const unsigned y_at = row * y_pitch + column * kSize, res_at = row * res_pitch + column * kSize;
+  float sx[kMT][kTurns];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int t = 0; t < kTurns; ++t)
+      sx[i][t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sx_rsrc, (row + i * 16 + t * kRows) * 4, 0, 0));
+  const Eight<float> sw = LoadEight<float, kVector>(sw_rsrc, column * 4, inside);
+  const Eight<T> bias = LoadEight<T, kVector>(bias_rsrc, column * kSize, inside);
+  const int write = (lane & 15) * (kNT * 64);
+#pragma unroll
+  for (int first = 0; first < kMT; first += kHeld) {
+    Eight<T> r[kHeld][kTurns];
+    if constexpr (kResidual) {
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t)
+          if (first + i < kMT) r[i][t] = LoadEight<T, kVector>(res_rsrc, res_at + ((first + i) * 16 + t * kRows) * res_pitch, inside);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = first; i < first + kHeld && i < kMT; ++i) {
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+        *reinterpret_cast<int4v*>(lds + write + ((j * 4 + (lane >> 4)) ^ (lane & kTurnMask)) * 16) = acc[i][j];
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int from = lane / kLanes + t * kRows;
+        int sum[8];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int4v part = *reinterpret_cast<const int4v*>(lds + from * (kNT * 64) + ((lane % kLanes * 2 + c) ^ (from & kTurnMask)) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[4 * c + e] = part[e];
+        }
+        float v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          v[c] = static_cast<float>(sum[c]) * (sx[i][t] * sw[c]) + bias[c];
+          if constexpr (kResidual) v[c] += r[i - first][t][c];
+        }
+        StoreEight<T, kVector>(y_rsrc, y_at + (i * 16 + t * kRows) * y_pitch, inside, v);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // registers: no more than 16 tokens at a time
+    }
+  }
+}
+
+// A block keeps a ring of kStages stages, each 64 k of a BM x BN tile's operands, and works through its tiles as one
+// sequence of stages: the first stages of the next tile are on their way while this one is finished.
+template <typename T, int BM, int BN, int kWM, int kWN, int kStages, int kBlocks>
+__global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs a, Tiles tiles) {
+  constexpr int kWaves = kWM * kWN;
+  constexpr int kMT = BM / (16 * kWM), kNT = BN / (16 * kWN);     // fragments of a wave
+  constexpr int kXDma = BM / (16 * kWaves), kWDma = BN / (16 * kWaves);  // wave copies of 16 rows per stage
+  constexpr int kDma = kXDma + kWDma;
+  constexpr int kStageBytes = (BM + BN) * kTileK;
+  static_assert(kXDma >= 1 && kWDma >= 1 && (kStages - 2) * kDma <= 63, "tile does not fit the wave layout");
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / kWN, wn = wave % kWN;
+
+  TileCursor tile, next;  // the tile being computed, and the one whose stages are being requested
+  tile.at = next.at = blockIdx.x >> 3;
+  tile.Place<BM, BN>(a, tiles);
+  if (tile.rows == 0) return;
+  next = tile;
+
+  // Staging: copy i of a wave fills rows 16 (i kWaves + wave) .. + 15, lane l the 16 bytes at row l >> 2, place l & 3.
+  // Place of a row's 16-byte chunk: chunk ^ Turn(row >> 2).  The 16 lanes whose reads the banks serve together - four
+  // rows of each multiple of four, not all of the same chunk - then lie in 16 different 16-byte columns of the 256
+  // bytes that the banks span.
+  const int chunk = (lane & 3) ^ Turn(lane >> 4);
+  unsigned x_off[kXDma], w_off[kWDma];
+#pragma unroll
+  for (int i = 0; i < kXDma; ++i)
+    x_off[i] = static_cast<unsigned>((i * kWaves + wave) * 16 + (lane >> 2)) * static_cast<unsigned>(a.x_stride);
+#pragma unroll
+  for (int i = 0; i < kWDma; ++i)
+    w_off[i] = static_cast<unsigned>((i * kWaves + wave) * 16 + (lane >> 2)) * static_cast<unsigned>(a.w_stride);
+  const int span = ((a.k + kTileK - 1) / kTileK + 1) / 2 * (2 * kTileK);  // k of a tile in whole pairs of stages
+  __amdgpu_buffer_rsrc_t x_rsrc, w_rsrc;
+  auto describe = [&]() {  // past the last tile: nothing, zeros arrive
+    x_rsrc = Descriptor(a.x + next.m0 * a.x_stride, next.rows ? (next.rows - 1) * a.x_stride + a.k : 0);
+    w_rsrc = Descriptor(a.w + next.n0 * a.w_stride, next.rows ? (next.columns - 1) * a.w_stride + a.k : 0);
+  };
+  describe();
+  int issue_k = 0;   // k of the next stage to be requested
+  int issue_at = 0;  // its place in the ring, bytes
+  unsigned issue_off = 0;
+  auto issue_begin = [&]() { issue_off = issue_k + chunk * 16 < a.k ? static_cast<unsigned>(issue_k + chunk * 16) : kOutside; };
+  auto issue_one = [&](auto i) {
+    constexpr int d = decltype(i)::value;
+    if constexpr (d < kXDma) DmaToLds(x_rsrc, x_off[d] + issue_off, lds + issue_at + (d * kWaves + wave) * 1024);
+    else DmaToLds(w_rsrc, w_off[d - kXDma] + issue_off, lds + issue_at + BM * kTileK + ((d - kXDma) * kWaves + wave) * 1024);
+  };
+  auto issue_end = [&]() {
+    issue_at = issue_at + kStageBytes == kStages * kStageBytes ? 0 : issue_at + kStageBytes;
+    issue_k += kTileK;
+    if (issue_k == span) {
+      issue_k = 0;
+      next.at += gridDim.x >> 3;
+      next.Place<BM, BN>(a, tiles);
+      describe();
+    }
+  };
+
+  // Fragments: lane l holds row l & 15, k 16 (l >> 4) .. + 15
+  const int frag = (lane & 15) * kTileK + ((lane >> 4) ^ Turn(lane >> 2)) * 16;
+  const int x_frag = wm * (BM / kWM) * kTileK + frag;
+  const int w_frag = (BM + wn * (BN / kWN)) * kTileK + frag;
+  int4v x[2][kMT], w[2][kNT];
+  int read_at = 0;
+  auto read_one = [&](auto set, auto i) {
+    constexpr int s = decltype(set)::value, d = decltype(i)::value;
+    if constexpr (d < kNT) w[s][d] = *reinterpret_cast<const int4v*>(lds + read_at + w_frag + d * 16 * kTileK);
+    else x[s][d - kNT] = *reinterpret_cast<const int4v*>(lds + read_at + x_frag + (d - kNT) * 16 * kTileK);
+  };
+  auto read_end = [&]() { read_at = read_at + kStageBytes == kStages * kStageBytes ? 0 : read_at + kStageBytes; };
+
+  int4v acc[kMT][kNT];
+  // Step s: the fragments of s are in registers.  Those of s + 1 are read, stage s + kStages is requested into the
+  // place of s (read by every wave before the last barrier), both between the products.
+  auto step = [&](auto set) {
+    constexpr int cur = decltype(set)::value;
+    // A request or a read at most between two products: a product occupies its unit for 16 cycles and the wave is free
+    // to issue for 12 of them; what does not fit there leaves the unit idle.
+    constexpr int kProducts = kMT * kNT, kReads = kMT + kNT, kSlots = kReads + kDma;
+    issue_begin();
+    Unrolled<0, kProducts>([&](auto t) {
+      constexpr int p = decltype(t)::value, i = p / kNT, j = p % kNT;
+      Mfma(w[cur][j], x[cur][i], acc[i][j]);
+      Unrolled<p * kSlots / kProducts, (p + 1) * kSlots / kProducts>([&](auto slot) {
+        constexpr int q = decltype(slot)::value;  // the requests evenly among the reads
+        constexpr int before = (q + 1) * kDma / kSlots;
+        if constexpr (q * kDma / kSlots != before) issue_one(std::integral_constant<int, before - 1>{});
+        else read_one(std::integral_constant<int, 1 - cur>{}, std::integral_constant<int, q - before>{});
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    issue_end();
+    read_end();
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kDma) : "memory");
+    __builtin_amdgcn_s_barrier();
+  };
+
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) {
+    issue_begin();
+    Unrolled<0, kDma>(issue_one);
+    issue_end();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kDma) : "memory");
+  __builtin_amdgcn_s_barrier();
+  Unrolled<0, kMT + kNT>([&](auto i) { read_one(std::integral_constant<int, 0>{}, i); });
+  read_end();
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kDma) : "memory");
+  __builtin_amdgcn_s_barrier();
+
+  while (true) {
+#pragma unroll
+    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        acc[i][j] = int4v{0, 0, 0, 0};
+        Pin(acc[i][j]);
+      }
+    SettleAccumulators();
+    for (int k = 0; k < span; k += 2 * kTileK) {  // the last stage may be zeros
+      step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+    }
+    SettleAccumulators();
+#pragma unroll
+    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) Pin(acc[i][j]);
+    int8_t* const mine = lds + kStages * kStageBytes + wave * (kNT * 1024);
+    if (!a.vector_rows) FinishWave<T, false, true>(a, tile, wm * (BM / kWM), wn * (BN / kWN), mine, acc);
+    else if (a.residual) FinishWave<T, true, true>(a, tile, wm * (BM / kWM), wn * (BN / kWN), mine, acc);
+    else FinishWave<T, true, false>(a, tile, wm * (BM / kWM), wn * (BN / kWN), mine, acc);
+    tile.at += gridDim.x >> 3;
+    tile.Place<BM, BN>(a, tiles);
+    if (tile.rows == 0) break;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may arrive in this LDS after the block has left it
+}
+
 int Status() {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : -1000 - static_cast<int>(e);
@@ -170,6 +543,34 @@ int LaunchSplit(const LinearArgs& a, hipStream_t stream) {
   return Status();
 }
 
+template <typename T, int BM, int BN, int kWM, int kWN, int kStages, int kBlocks>
+int LaunchTile(const LinearArgs& a, hipStream_t stream) {
+  const long long tiles_m = (a.m + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN;
+  if (tiles_m * tiles_n > (1ll << 30)) return -3;
+  const Tiles tiles{static_cast<unsigned>(tiles_m), static_cast<unsigned>(tiles_n), static_cast<unsigned>((tiles_m * tiles_n + 7) / 8)};
+  constexpr int kLds = kStages * (BM + BN) * kTileK + 16 * BN * kWM * 4;
+  constexpr unsigned kPerXcd = 32 * kBlocks;  // blocks that an XCD's 32 CUs hold
+  if (kLds > 65536) {
+    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&TileKernel<T, BM, BN, kWM, kWN, kStages, kBlocks>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (once != hipSuccess) return -1000 - static_cast<int>(once);
+  }
+  hipLaunchKernelGGL((TileKernel<T, BM, BN, kWM, kWN, kStages, kBlocks>), dim3(8 * (tiles.run < kPerXcd ? tiles.run : kPerXcd)),
+                     dim3(64 * kWM * kWN), kLds, stream, a, tiles);
+  return Status();
+}
+
+template <typename T>
+int Launch(const LinearArgs& a, hipStream_t st) {
+  const bool aligned = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.x_stride | a.w_stride | a.k) & 15) == 0;
+  constexpr long long kMost = 1 << 20;  // 256 rows of a tile stay below 2^30 bytes
+  if (aligned && a.x_stride <= kMost && a.w_stride <= kMost && a.y_stride <= kMost && a.residual_stride <= kMost && a.m > 64) {
+    const long long big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
+    return big >= 128 ? LaunchTile<T, 256, 256, 2, 2, 4, 1>(a, st) : LaunchTile<T, 128, 128, 2, 2, 4, 2>(a, st);
+  }
+  return a.m <= 16 ? LaunchSplit<1, 1, 8>(a, st) : LaunchSplit<4, 4, 4>(a, st);
+}
+
 }  // namespace
 
 extern "C" int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, const void* w_scale, const void* bias,
@@ -179,9 +580,13 @@ extern "C" int tca_int8_linear_launch(const void* x, const void* x_scale, const 
   if (!x || !x_scale || !w || !w_scale || !y || m <= 0 || n <= 0 || k <= 0) return -1;
   if (dtype != tca::kF32 && dtype != tca::kF16 && dtype != tca::kBF16) return -2;
   if (k > 131071) return -3;
+  const bool vector_rows = ((reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias)) & 15) == 0 &&
+                           ((n | y_stride | (residual ? residual_stride : 0)) & 7) == 0 &&
+                           ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 15) == 0;
   LinearArgs a{static_cast<const int8_t*>(x),  static_cast<const float*>(x_scale), static_cast<const int8_t*>(w),
                static_cast<const float*>(w_scale), bias, residual, y, m, n, x_stride, w_stride, residual_stride, y_stride,
-               static_cast<int>(k), dtype};
+               static_cast<int>(k), dtype, vector_rows};
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return m <= 16 ? LaunchSplit<1, 1, 8>(a, st) : LaunchSplit<4, 4, 4>(a, st);
+  if (dtype == tca::kF32) return Launch<float>(a, st);
+  return dtype == tca::kF16 ? Launch<_Float16>(a, st) : Launch<Bf16>(a, st);
 }
