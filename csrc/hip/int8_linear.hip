@@ -21,6 +21,7 @@
 //              32 x 32 x 32 and win although they issue twice as often (443 against 476 us at the same stage of tuning).
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -45,30 +46,64 @@ struct LinearArgs {
   int vector_rows;  // every eighth output starts at a multiple of 16 bytes, in y and the residual, and n % 8 == 0
 };
 
-__device__ __forceinline__ float Load(const void* p, long long at, int dtype) {
-  if (dtype == tca::kF32) return static_cast<const float*>(p)[at];
-  if (dtype == tca::kF16) return static_cast<float>(static_cast<const _Float16*>(p)[at]);
-  return __uint_as_float(static_cast<unsigned>(static_cast<const unsigned short*>(p)[at]) << 16);
+struct Bf16 {
+  unsigned short bits;
+};
+__device__ __forceinline__ float ToFloat(float v) { return v; }
+__device__ __forceinline__ float ToFloat(_Float16 v) { return static_cast<float>(v); }
+__device__ __forceinline__ float ToFloat(Bf16 v) { return __uint_as_float(static_cast<unsigned>(v.bits) << 16); }
+template <typename T> __device__ __forceinline__ T FromFloat(float v);
+template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
+template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) { return static_cast<_Float16>(v); }
+template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
+  return Bf16{__builtin_bit_cast(unsigned short, static_cast<__bf16>(v))};
 }
 
-__device__ __forceinline__ void Store(void* p, long long at, int dtype, float v) {
-  if (dtype == tca::kF32) static_cast<float*>(p)[at] = v;
-  else if (dtype == tca::kF16) static_cast<_Float16*>(p)[at] = static_cast<_Float16>(v);
-  else static_cast<unsigned short*>(p)[at] = __builtin_bit_cast(unsigned short, static_cast<__bf16>(v));
-}
-
-// one lane's accumulators: outputs n .. n + 3 of token m
-__device__ __forceinline__ void Finish(const LinearArgs& a, long long m, long long n, int4v acc) {
-  if (m >= a.m) return;
+// one lane's sums: outputs n .. n + 3 of token m
+template <typename T>
+__device__ __forceinline__ void FinishFour(const LinearArgs& a, long long m, long long n, int4v sum) {
+  struct alignas(4 * sizeof(T)) Four {
+    T v[4];
+  };
+  const T* bias = static_cast<const T*>(a.bias) + n;
+  const T* residual = static_cast<const T*>(a.residual) + m * a.residual_stride + n;
+  T* y = static_cast<T*>(a.y) + m * a.y_stride + n;
   const float sx = a.x_scale[m];
+  if (a.vector_rows) {  // n % 4 == 0, so all four are there
+    const float4 sw = *reinterpret_cast<const float4*>(a.w_scale + n);
+    float v[4] = {static_cast<float>(sum[0]) * (sx * sw.x), static_cast<float>(sum[1]) * (sx * sw.y),
+                  static_cast<float>(sum[2]) * (sx * sw.z), static_cast<float>(sum[3]) * (sx * sw.w)};
+    if (a.bias) {
+      const Four b = *reinterpret_cast<const Four*>(bias);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (n + i >= a.n) return;
-    float v = static_cast<float>(acc[i]) * (sx * a.w_scale[n + i]);
-    if (a.bias) v += Load(a.bias, n + i, a.dtype);
-    if (a.residual) v += Load(a.residual, m * a.residual_stride + n + i, a.dtype);
-    Store(a.y, m * a.y_stride + n + i, a.dtype, v);
+      for (int i = 0; i < 4; ++i) v[i] += ToFloat(b.v[i]);
+    }
+    if (a.residual) {
+      const Four r = *reinterpret_cast<const Four*>(residual);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += ToFloat(r.v[i]);
+    }
+    Four out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out.v[i] = FromFloat<T>(v[i]);
+    *reinterpret_cast<Four*>(y) = out;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= a.n) return;
+      float v = static_cast<float>(sum[i]) * (sx * a.w_scale[n + i]);
+      if (a.bias) v += ToFloat(bias[i]);
+      if (a.residual) v += ToFloat(residual[i]);
+      y[i] = FromFloat<T>(v);
+    }
   }
+}
+
+__device__ __forceinline__ void Finish(const LinearArgs& a, long long m, long long n, int4v sum) {
+  if (m >= a.m || n >= a.n) return;
+  if (a.dtype == tca::kF32) FinishFour<float>(a, m, n, sum);
+  else if (a.dtype == tca::kF16) FinishFour<_Float16>(a, m, n, sum);
+  else FinishFour<Bf16>(a, m, n, sum);
 }
 
 // 16 bytes of a row from k on; zeros past the row's end (bytes there may belong to nobody)
@@ -88,7 +123,7 @@ __device__ __forceinline__ int4v LoadTail(const int8_t* row, int k, int end) {
 constexpr int kStep = 128;  // k per wave and step: a lane reads 32 consecutive bytes, four lanes a whole cache line
 
 // Block tile: 16 kMT tokens x 16 kNT outputs, k split over kWaves waves.
-template <int kMT, int kNT, int kWaves>
+template <int kMT, int kNT, int kWaves, int kAhead>
 __global__ __launch_bounds__(64 * kWaves) void SplitKernel(LinearArgs a, long long m_first, unsigned tiles_n) {
   extern __shared__ __attribute__((aligned(16))) int4v parts[];  // [kWaves][kMT * kNT][64]
   const unsigned tile_m = blockIdx.x / tiles_n;
@@ -116,19 +151,30 @@ __global__ __launch_bounds__(64 * kWaves) void SplitKernel(LinearArgs a, long lo
     for (int j = 0; j < kNT; ++j) acc[i][j] = int4v{0, 0, 0, 0};
   const int whole = a.k / kStep;
   const int at = (lane >> 4) * 32;
-  for (int s = wave; s < whole; s += kWaves) {
-    int4v x[kMT][2], w[kNT][2];
+  auto steps = [&](int s, auto count) {  // `count` steps of this wave from s on, all loads before the first product
+    constexpr int kCount = decltype(count)::value;
+    int4v x[kCount][kMT][2], w[kCount][kNT][2];
 #pragma unroll
-    for (int j = 0; j < kNT; ++j) __builtin_memcpy(w[j], wr[j] + s * kStep + at, 32);
+    for (int u = 0; u < kCount; ++u) {
+      const int k = (s + u * kWaves) * kStep + at;
 #pragma unroll
-    for (int i = 0; i < kMT; ++i) __builtin_memcpy(x[i], xr[i] + s * kStep + at, 32);
+      for (int j = 0; j < kNT; ++j) __builtin_memcpy(w[u][j], wr[j] + k, 32);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int i = 0; i < kMT; ++i) __builtin_memcpy(x[u][i], xr[i] + k, 32);
+    }
 #pragma unroll
-      for (int i = 0; i < kMT; ++i)
+    for (int u = 0; u < kCount; ++u)
 #pragma unroll
-        for (int j = 0; j < kNT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j][h], x[i][h], acc[i][j], 0, 0, 0);
-  }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < kMT; ++i)
+#pragma unroll
+          for (int j = 0; j < kNT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][j][h], x[u][i][h], acc[i][j], 0, 0, 0);
+  };
+  int s = wave;
+  for (; s + (kAhead - 1) * kWaves < whole; s += kAhead * kWaves) steps(s, std::integral_constant<int, kAhead>{});
+  for (; s < whole; s += kWaves) steps(s, std::integral_constant<int, 1>{});
   if (whole * kStep < a.k && wave == whole % kWaves) {  // the last, partial step
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -157,19 +203,116 @@ __global__ __launch_bounds__(64 * kWaves) void SplitKernel(LinearArgs a, long lo
   }
 }
 
-// ---- Epilogue of a tile: results leave straight from the accumulators ----------------------------------------------
+// An offset behind every descriptor's end, also with a row's offset added: the DMA writes zeros for it, loads give zeros,
+// stores are dropped.  The host keeps the rows of a tile below 2^30 bytes.
+constexpr unsigned kOutside = 0x80000000u;
 
-struct Bf16 {
-  unsigned short bits;
-};
-__device__ __forceinline__ float ToFloat(float v) { return v; }
-__device__ __forceinline__ float ToFloat(_Float16 v) { return static_cast<float>(v); }
-__device__ __forceinline__ float ToFloat(Bf16 v) { return __uint_as_float(static_cast<unsigned>(v.bits) << 16); }
-template <typename T> __device__ __forceinline__ T FromFloat(float v);
-template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
-template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) { return static_cast<_Float16>(v); }
-template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
-  return Bf16{__builtin_bit_cast(unsigned short, static_cast<__bf16>(v))};
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t Descriptor(const void* p, long long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(p ? bytes : 0), 0x00020000);
+}
+
+using lds_ptr_t = __attribute__((address_space(3))) void*;
+
+// Wave-wide copy global -> LDS, 16 bytes per lane, to lds + 16 * lane
+__device__ __forceinline__ void DmaToLds(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int8_t* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, reinterpret_cast<lds_ptr_t>(reinterpret_cast<uintptr_t>(lds)), 16,
+                                           static_cast<int>(offset), 0, 0, 0);
+}
+
+template <int kFirst, int kLast, typename F>
+__device__ __forceinline__ void Unrolled(F&& f) {
+  if constexpr (kFirst < kLast) {
+    f(std::integral_constant<int, kFirst>{});
+    Unrolled<kFirst + 1, kLast>(f);
+  }
+}
+
+// The same split over waves, operands through LDS: each wave keeps a ring of kStages steps of its own, filled by DMA.
+// The registers' way has every lane of a quarter wave in another row, so each 16 bytes are a cache lookup of their own
+// and a CU takes in 14 bytes per cycle however the loads are arranged; the DMA's lanes go along the rows, eight to a
+// 128-byte line.  No barrier until the sums meet.
+template <int kMT, int kNT, int kWaves, int kStages>
+__global__ __launch_bounds__(64 * kWaves) void SplitDmaKernel(LinearArgs a, long long m_first, unsigned tiles_n) {
+  constexpr int kXDma = 2 * kMT, kDma = 2 * (kMT + kNT);  // copies of 8 rows
+  constexpr int kStageBytes = kDma * 1024;
+  static_assert(kStages * kStageBytes >= kMT * kNT * 1024, "the sums meet in the ring's place");
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+  const unsigned tile_m = blockIdx.x / tiles_n;
+  const unsigned tile_n = blockIdx.x - tile_m * tiles_n;
+  const long long m0 = m_first + static_cast<long long>(tile_m) * (16 * kMT);
+  const long long n0 = static_cast<long long>(tile_n) * (16 * kNT);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int8_t* const ring = lds + wave * (kStages * kStageBytes);
+  const int x_rows = static_cast<int>(a.m - m0 < 16 * kMT ? a.m - m0 : 16 * kMT);
+  const int w_rows = static_cast<int>(a.n - n0 < 16 * kNT ? a.n - n0 : 16 * kNT);
+  const auto x_rsrc = Descriptor(a.x + m0 * a.x_stride, (x_rows - 1) * a.x_stride + a.k);
+  const auto w_rsrc = Descriptor(a.w + n0 * a.w_stride, (w_rows - 1) * a.w_stride + a.k);
+  // Copy i brings rows 8 i .. 8 i + 7 of 128 bytes; a row's chunk c lies at place c ^ ((row >> 1) & 7), which keeps the
+  // lanes whose fragment reads the banks serve together in different columns.
+  const unsigned x_row = static_cast<unsigned>(lane >> 3) * static_cast<unsigned>(a.x_stride);
+  const unsigned w_row = static_cast<unsigned>(lane >> 3) * static_cast<unsigned>(a.w_stride);
+  const int chunk = (lane & 7) ^ (lane >> 4);  // of even copies; 4 further on (exclusive or) in odd ones
+  auto issue = [&](int s, int stage) {
+    unsigned k[2];
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const int at = s * kStep + (chunk ^ (4 * odd)) * 16;
+      k[odd] = at < a.k ? static_cast<unsigned>(at) : kOutside;
+    }
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) {
+      int8_t* to = ring + stage * kStageBytes + i * 1024;
+      if (i < kXDma) DmaToLds(x_rsrc, x_row + static_cast<unsigned>(i * 8 * a.x_stride) + k[i & 1], to);
+      else DmaToLds(w_rsrc, w_row + static_cast<unsigned>((i - kXDma) * 8 * a.w_stride) + k[i & 1], to);
+    }
+  };
+  int4v acc[kMT][kNT];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) acc[i][j] = int4v{0, 0, 0, 0};
+  const int steps = (a.k + kStep - 1) / kStep;
+  const int frag = (lane & 15) * kStep + ((lane >> 4) ^ ((lane >> 1) & 7)) * 16;
+  int ahead = wave;
+#pragma unroll
+  for (int stage = 0; stage < kStages; ++stage, ahead += kWaves) issue(ahead, stage);  // past the end: zeros
+  int stage = 0;
+  for (int s = wave; s < steps; s += kWaves) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kDma) : "memory");
+    int4v x[kMT][2], w[kNT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int8_t* from = ring + stage * kStageBytes + (frag ^ (h * 64));
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) x[i][h] = *reinterpret_cast<const int4v*>(from + i * 16 * kStep);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) w[j][h] = *reinterpret_cast<const int4v*>(from + (kMT + j) * 16 * kStep);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before it is filled again
+    issue(ahead, stage);
+    ahead += kWaves;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j][h], x[i][h], acc[i][j], 0, 0, 0);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  int4v* parts = reinterpret_cast<int4v*>(ring);  // own place: every arrival has been waited for
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) parts[(i * kNT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int f = wave; f < kMT * kNT; f += kWaves) {
+    int4v sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) sum += *reinterpret_cast<const int4v*>(lds + v * (kStages * kStageBytes) + (f * 64 + lane) * 16);
+    Finish(a, m0 + (f / kNT) * 16 + (lane & 15), n0 + (f % kNT) * 16 + (lane >> 4) * 4, sum);
+  }
 }
 
 // Eight consecutive values as they lie in memory.  kVector: at a multiple of 16 bytes, all inside or all outside a
@@ -185,14 +328,6 @@ struct Eight {
 };
 
 using uint4v = __attribute__((ext_vector_type(4))) unsigned;
-
-// An offset behind every descriptor's end, also with a row's offset added: the DMA writes zeros for it, loads give zeros,
-// stores are dropped.  The host keeps the rows of a tile below 2^30 bytes.
-constexpr unsigned kOutside = 0x80000000u;
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t Descriptor(const void* p, long long bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(p ? bytes : 0), 0x00020000);
-}
 
 // `inside` of the eight lie in the row: all or none of them with kVector
 template <typename T, bool kVector>
@@ -243,15 +378,7 @@ __device__ __forceinline__ void StoreEight(__amdgpu_buffer_rsrc_t rsrc, unsigned
 
 // ---- TileKernel ---------------------------------------------------------------------------------------------------
 
-using lds_ptr_t = __attribute__((address_space(3))) void*;
-
 constexpr int kTileK = 64;  // k per stage: an LDS row of an operand is 64 bytes, one MFMA deep
-
-// Wave-wide copy global -> LDS, 16 bytes per lane, to lds + 16 * lane
-__device__ __forceinline__ void DmaToLds(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int8_t* lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, reinterpret_cast<lds_ptr_t>(reinterpret_cast<uintptr_t>(lds)), 16,
-                                           static_cast<int>(offset), 0, 0, 0);
-}
 
 // The tiles of a block: each of the 8 XCDs (consecutive blocks go round them) has a contiguous run of tiles, ordered in
 // bands of kBand tile rows, so that the tiles an XCD works on at a time share operands in its L2; its blocks take them
@@ -295,14 +422,6 @@ __device__ __forceinline__ void Mfma(int4v w, int4v x, int4v& acc) {
 // touch the accumulators (16 cycles of the instruction and its write) stands here.
 __device__ __forceinline__ void SettleAccumulators() { asm volatile("s_nop 15\n\ts_nop 7"); }
 __device__ __forceinline__ void Pin(int4v& acc) { asm volatile("" : "+a"(acc)); }  // ordered with the other asm
-
-template <int kFirst, int kLast, typename F>
-__device__ __forceinline__ void Unrolled(F&& f) {
-  if constexpr (kFirst < kLast) {
-    f(std::integral_constant<int, kFirst>{});
-    Unrolled<kFirst + 1, kLast>(f);
-  }
-}
 
 // 0, 2, 3, 1 for the low two bits 0, 1, 2, 3
 __device__ __forceinline__ int Turn(int v) { return ((v ^ (v >> 1)) & 1) * 2 + ((v >> 1) & 1); }
@@ -459,19 +578,19 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
   // place of s (read by every wave before the last barrier), both between the products.
   auto step = [&](auto set) {
     constexpr int cur = decltype(set)::value;
-    // A request or a read at most between two products: a product occupies its unit for 16 cycles and the wave is free
-    // to issue for 12 of them; what does not fit there leaves the unit idle.
-    constexpr int kProducts = kMT * kNT, kReads = kMT + kNT, kSlots = kReads + kDma;
+    // A request or a read or two between two products: a product occupies its unit for 16 cycles and the wave is free to
+    // issue for 12 of them; what does not fit there leaves the unit idle.  The reads come first, so that the last of
+    // them has arrived when the step ends.
+    constexpr int kProducts = kMT * kNT, kReads = kMT + kNT, kReadPart = kProducts / 2, kAskPart = kProducts * 3 / 8;
     issue_begin();
     Unrolled<0, kProducts>([&](auto t) {
       constexpr int p = decltype(t)::value, i = p / kNT, j = p % kNT;
       Mfma(w[cur][j], x[cur][i], acc[i][j]);
-      Unrolled<p * kSlots / kProducts, (p + 1) * kSlots / kProducts>([&](auto slot) {
-        constexpr int q = decltype(slot)::value;  // the requests evenly among the reads
-        constexpr int before = (q + 1) * kDma / kSlots;
-        if constexpr (q * kDma / kSlots != before) issue_one(std::integral_constant<int, before - 1>{});
-        else read_one(std::integral_constant<int, 1 - cur>{}, std::integral_constant<int, q - before>{});
-      });
+      if constexpr (p < kReadPart)
+        Unrolled<p * kReads / kReadPart, (p + 1) * kReads / kReadPart>(
+            [&](auto d) { read_one(std::integral_constant<int, 1 - cur>{}, d); });
+      if constexpr (p >= kReadPart && p < kReadPart + kAskPart)
+        Unrolled<(p - kReadPart) * kDma / kAskPart, (p - kReadPart + 1) * kDma / kAskPart>(issue_one);
       __builtin_amdgcn_sched_barrier(0);
     });
     issue_end();
@@ -522,23 +641,70 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may arrive in this LDS after the block has left it
 }
 
+// Rows that do not start at multiples of 16 bytes are copied to rows that do, zeros behind them: the DMA moves whole
+// 16-byte pieces.  x's rows come first, w's behind them.
+__global__ __launch_bounds__(256) void PadKernel(LinearArgs a, int8_t* __restrict__ to, int pieces) {
+  const long long count = (a.m + a.n) * pieces;
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<long long>(gridDim.x) * 256) {
+    const long long row = count >> 31 ? i / pieces : static_cast<unsigned>(i) / static_cast<unsigned>(pieces);
+    const int k = static_cast<int>(i - row * pieces) * 16;
+    const int8_t* from = row < a.m ? a.x + row * a.x_stride : a.w + (row - a.m) * a.w_stride;
+    *reinterpret_cast<int4v*>(to + i * 16) = LoadTail(from, k, a.k);
+  }
+}
+
 int Status() {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : -1000 - static_cast<int>(e);
 }
 
+// More than 64 KB of LDS has to be allowed, once for each kernel and device.
+template <auto* kKernel>
+int AllowLds(int bytes) {
+  static std::atomic<uint64_t> allowed{0};
+  if (bytes <= 65536) return 0;
+  int device = 0;
+  hipError_t e = hipGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (e == hipSuccess && !(allowed.load(std::memory_order_relaxed) & bit)) {
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == hipSuccess) allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return e == hipSuccess ? 0 : -1000 - static_cast<int>(e);
+}
+
 // A grid holds fewer than 2^32 threads: tokens beyond that go to further launches.
-template <int kMT, int kNT, int kWaves>
+template <int kMT, int kNT, int kWaves, int kAhead>
 int LaunchSplit(const LinearArgs& a, hipStream_t stream) {
   const long long tiles_n = (a.n + 16 * kNT - 1) / (16 * kNT);
   constexpr long long kMostBlocks = (1ll << 31) / (64 * kWaves);
   if (tiles_n > kMostBlocks) return -3;
   const long long most_m = kMostBlocks / tiles_n * (16 * kMT);
+  constexpr int kLds = kWaves * kMT * kNT * 1024;
+  static_assert(kLds <= 65536, "more would have to be asked for");
   for (long long m = 0; m < a.m; m += most_m) {
     const long long left = a.m - m < most_m ? a.m - m : most_m;
     const long long blocks = (left + 16 * kMT - 1) / (16 * kMT) * tiles_n;
-    hipLaunchKernelGGL((SplitKernel<kMT, kNT, kWaves>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),
-                       kWaves * kMT * kNT * 1024, stream, a, m, static_cast<unsigned>(tiles_n));
+    hipLaunchKernelGGL((SplitKernel<kMT, kNT, kWaves, kAhead>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),
+                       kLds, stream, a, m, static_cast<unsigned>(tiles_n));
+  }
+  return Status();
+}
+
+template <int kMT, int kNT, int kWaves, int kStages>
+int LaunchSplitDma(const LinearArgs& a, hipStream_t stream) {
+  const long long tiles_n = (a.n + 16 * kNT - 1) / (16 * kNT);
+  constexpr long long kMostBlocks = (1ll << 31) / (64 * kWaves);
+  constexpr int kLds = kWaves * kStages * (kMT + kNT) * 2048;
+  static_assert(kLds <= 160 * 1024 && (kStages - 1) * 2 * (kMT + kNT) <= 63, "ring too large");
+  if (tiles_n > kMostBlocks) return -3;
+  if (const int rc = AllowLds<&SplitDmaKernel<kMT, kNT, kWaves, kStages>>(kLds)) return rc;
+  const long long most_m = kMostBlocks / tiles_n * (16 * kMT);
+  for (long long m = 0; m < a.m; m += most_m) {
+    const long long left = a.m - m < most_m ? a.m - m : most_m;
+    const long long blocks = (left + 16 * kMT - 1) / (16 * kMT) * tiles_n;
+    hipLaunchKernelGGL((SplitDmaKernel<kMT, kNT, kWaves, kStages>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), kLds,
+                       stream, a, m, static_cast<unsigned>(tiles_n));
   }
   return Status();
 }
@@ -549,44 +715,101 @@ int LaunchTile(const LinearArgs& a, hipStream_t stream) {
   if (tiles_m * tiles_n > (1ll << 30)) return -3;
   const Tiles tiles{static_cast<unsigned>(tiles_m), static_cast<unsigned>(tiles_n), static_cast<unsigned>((tiles_m * tiles_n + 7) / 8)};
   constexpr int kLds = kStages * (BM + BN) * kTileK + 16 * BN * kWM * 4;
+  static_assert(kBlocks * kLds <= 160 * 1024, "a CU's LDS");
   constexpr unsigned kPerXcd = 32 * kBlocks;  // blocks that an XCD's 32 CUs hold
-  if (kLds > 65536) {
-    static const hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&TileKernel<T, BM, BN, kWM, kWN, kStages, kBlocks>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-    if (once != hipSuccess) return -1000 - static_cast<int>(once);
-  }
+  if (const int rc = AllowLds<&TileKernel<T, BM, BN, kWM, kWN, kStages, kBlocks>>(kLds)) return rc;
   hipLaunchKernelGGL((TileKernel<T, BM, BN, kWM, kWN, kStages, kBlocks>), dim3(8 * (tiles.run < kPerXcd ? tiles.run : kPerXcd)),
                      dim3(64 * kWM * kWN), kLds, stream, a, tiles);
   return Status();
 }
 
+bool Aligned(const void* x, const void* w, long long x_stride, long long w_stride, long long k) {
+  return ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | x_stride | w_stride | k) & 15) == 0;
+}
+
+// Descriptors hold 32-bit offsets: 256 rows of a tile have to stay below 2^30 bytes.
+constexpr long long kMostStride = 1 << 20;
+
+// Copying the operands to aligned rows costs their bytes twice and a launch; below this the kernel that reads rows at
+// any address is as fast.
+bool Pads(long long m, long long n, long long k) { return m > 32 && m * n > (1ll << 28) / k; }
+
+int PaddedRow(long long k) { return static_cast<int>((k + 15) / 16 * 16); }
+
+// The largest tile that leaves no more than a quarter of the 256 CUs idle, else the smallest: what a CU takes in per
+// output falls with the tile's sides, but half the CUs take in half the bytes per second.
 template <typename T>
-int Launch(const LinearArgs& a, hipStream_t st) {
-  const bool aligned = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.w) | a.x_stride | a.w_stride | a.k) & 15) == 0;
-  constexpr long long kMost = 1 << 20;  // 256 rows of a tile stay below 2^30 bytes
-  if (aligned && a.x_stride <= kMost && a.w_stride <= kMost && a.y_stride <= kMost && a.residual_stride <= kMost && a.m > 64) {
-    const long long big = ((a.m + 255) / 256) * ((a.n + 255) / 256);
-    return big >= 128 ? LaunchTile<T, 256, 256, 2, 2, 4, 1>(a, st) : LaunchTile<T, 128, 128, 2, 2, 4, 2>(a, st);
+int LaunchAligned(const LinearArgs& a, hipStream_t st) {
+  auto fills = [&](long long bm, long long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) >= 192; };
+  if (a.m > 64) {
+    if (fills(256, 256)) return LaunchTile<T, 256, 256, 2, 2, 4, 1>(a, st);
+    if (fills(256, 128)) return LaunchTile<T, 256, 128, 2, 2, 4, 1>(a, st);
+    if (fills(128, 128)) return LaunchTile<T, 128, 128, 2, 2, 4, 2>(a, st);
   }
-  return a.m <= 16 ? LaunchSplit<1, 1, 8>(a, st) : LaunchSplit<4, 4, 4>(a, st);
+  if (a.m > 32 && fills(64, 64)) return LaunchSplitDma<4, 4, 8, 1>(a, st);
+  if (a.m > 16) {
+    if (fills(32, 64)) return LaunchSplitDma<2, 4, 8, 1>(a, st);
+    if (fills(32, 32)) return LaunchSplitDma<2, 2, 4, 2>(a, st);
+    if (fills(32, 16)) return LaunchSplitDma<2, 1, 8, 2>(a, st);
+  }
+  if (fills(16, 64)) return LaunchSplitDma<1, 4, 8, 1>(a, st);
+  if (fills(16, 32)) return LaunchSplitDma<1, 2, 8, 2>(a, st);
+  // waves by the length of k: each has a few steps of 128
+  if (a.k > 8192) return LaunchSplitDma<1, 1, 16, 2>(a, st);
+  return a.k > 1024 ? LaunchSplitDma<1, 1, 8, 2>(a, st) : LaunchSplitDma<1, 1, 4, 2>(a, st);
+}
+
+int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
+  auto fills = [&](long long bm, long long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) >= 192; };
+  if (a.m > 32 && fills(64, 64)) return LaunchSplit<4, 4, 4, 1>(a, st);
+  if (a.m > 16 && fills(32, 32)) return LaunchSplit<2, 2, 8, 1>(a, st);
+  return LaunchSplit<1, 1, 8, 2>(a, st);
+}
+
+int Launch(LinearArgs a, void* workspace, hipStream_t st) {
+  if (!Aligned(a.x, a.w, a.x_stride, a.w_stride, a.k)) {
+    if (!Pads(a.m, a.n, a.k)) return LaunchUnaligned(a, st);
+    if (!workspace) return -4;
+    const int row = PaddedRow(a.k);
+    const long long blocks = ((a.m + a.n) * (row / 16) + 255) / 256;
+    hipLaunchKernelGGL(PadKernel, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, a,
+                       static_cast<int8_t*>(workspace), row / 16);
+    a.x = static_cast<const int8_t*>(workspace);
+    a.w = a.x + a.m * row;
+    a.x_stride = a.w_stride = row;
+    a.k = row;
+  }
+  if (a.x_stride > kMostStride || a.w_stride > kMostStride || a.y_stride > kMostStride || a.residual_stride > kMostStride)
+    return LaunchUnaligned(a, st);
+  if (a.dtype == tca::kF32) return LaunchAligned<float>(a, st);
+  return a.dtype == tca::kF16 ? LaunchAligned<_Float16>(a, st) : LaunchAligned<Bf16>(a, st);
 }
 
 }  // namespace
 
-extern "C" int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, const void* w_scale, const void* bias,
-                                      const void* residual, void* y, int dtype, long long m, long long n, long long k,
-                                      long long x_stride, long long w_stride, long long residual_stride,
-                                      long long y_stride, void* stream) {
+extern "C" {
+
+// Bytes of workspace (at a multiple of 16) that a launch with these operands needs; mostly 0.
+long long tca_int8_linear_workspace_bytes(const void* x, const void* w, long long m, long long n, long long k, long long x_stride,
+                                          long long w_stride) {
+  if (m <= 0 || n <= 0 || k <= 0 || Aligned(x, w, x_stride, w_stride, k) || !Pads(m, n, k)) return 0;
+  return (m + n) * PaddedRow(k);
+}
+
+int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, const void* w_scale, const void* bias,
+                           const void* residual, void* y, int dtype, long long m, long long n, long long k,
+                           long long x_stride, long long w_stride, long long residual_stride, long long y_stride,
+                           void* workspace, void* stream) {
   if (!x || !x_scale || !w || !w_scale || !y || m <= 0 || n <= 0 || k <= 0) return -1;
   if (dtype != tca::kF32 && dtype != tca::kF16 && dtype != tca::kBF16) return -2;
-  if (k > 131071) return -3;
-  const bool vector_rows = ((reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias)) & 15) == 0 &&
-                           ((n | y_stride | (residual ? residual_stride : 0)) & 7) == 0 &&
-                           ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 15) == 0;
-  LinearArgs a{static_cast<const int8_t*>(x),  static_cast<const float*>(x_scale), static_cast<const int8_t*>(w),
-               static_cast<const float*>(w_scale), bias, residual, y, m, n, x_stride, w_stride, residual_stride, y_stride,
-               static_cast<int>(k), dtype, vector_rows};
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == tca::kF32) return Launch<float>(a, st);
-  return dtype == tca::kF16 ? Launch<_Float16>(a, st) : Launch<Bf16>(a, st);
+  if (k > 131071 || (reinterpret_cast<uintptr_t>(workspace) & 15)) return -3;
+  const bool vector_rows = ((reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias) |
+                             reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 15) == 0 &&
+                           ((n | y_stride | (residual ? residual_stride : 0)) & 7) == 0;
+  const LinearArgs a{static_cast<const int8_t*>(x), static_cast<const float*>(x_scale), static_cast<const int8_t*>(w),
+                     static_cast<const float*>(w_scale), bias, residual, y, m, n, x_stride, w_stride,
+                     residual ? residual_stride : 0, y_stride, static_cast<int>(k), dtype, vector_rows};
+  return Launch(a, workspace, static_cast<hipStream_t>(stream));
 }
+
+}  // extern "C"

@@ -131,5 +131,7 @@ int tca_int8_dequantize_launch(const void* q, const void* scale, void* out, int 
 int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, const void* w_scale, const void* bias,
                            const void* residual, void* y, int dtype, long long m, long long n, long long k,
                            long long x_stride, long long w_stride, long long residual_stride, long long y_stride,
-                           void* stream);
+                           void* workspace, void* stream);
+long long tca_int8_linear_workspace_bytes(const void* x, const void* w, long long m, long long n, long long k, long long x_stride,
+                                          long long w_stride);
 }

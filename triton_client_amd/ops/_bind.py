@@ -155,7 +155,10 @@ def install(lib):
     lib.tca_int8_linear_launch.restype = c_int
     lib.tca_int8_linear_launch.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
                                            c_longlong, c_longlong, c_longlong, c_longlong, c_longlong, c_longlong,
-                                           c_longlong, c_void_p]
+                                           c_longlong, c_void_p, c_void_p]
+    lib.tca_int8_linear_workspace_bytes.restype = c_longlong
+    lib.tca_int8_linear_workspace_bytes.argtypes = [c_void_p, c_void_p, c_longlong, c_longlong, c_longlong, c_longlong,
+                                                    c_longlong]
     install_rt(lib)
 
 

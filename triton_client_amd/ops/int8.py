@@ -29,43 +29,35 @@ instead of a number.  The reference has no model code (its models run in the ser
 
 from __future__ import annotations
 
+import torch
+
 from ._device import check, lib
 
 # 128 * 128 * k has to stay below 2^31
 MAX_K = 131071
 MAX_WIDTH = 1 << 29
 
-_TYPE_CODE = None
-
-
-def _codes():
-    import torch
-
-    global _TYPE_CODE
-    if _TYPE_CODE is None:
-        _TYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    return _TYPE_CODE
+_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 def _float_code(t, name):
-    code = _codes().get(t.dtype)
+    code = _CODES.get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be an fp16, bf16 or fp32 tensor")
     return code
 
 
 def _output_code(dtype):
-    code = _codes().get(dtype)
+    code = _CODES.get(dtype)
     if code is None:
         raise TypeError("dtype must be torch.float16, torch.bfloat16 or torch.float32")
     return code
 
 
 def _refuse_gradients(*operands):
-    import torch
-
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in operands):
-        raise ValueError("8-bit operators have no gradient: detach the operands or call under torch.no_grad()")
+    for t in operands:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("8-bit operators have no gradient: detach the operands or call under torch.no_grad()")
 
 
 def _same_device(first, *others):
@@ -138,16 +130,23 @@ def _check_apart(outputs, inputs):
                 raise ValueError(f"{name} overlaps {other}")
 
 
-def _launch(what, device, *args):
-    import torch
+# the handle alone, where torch gives it: an object around it costs more than the checks of a call
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
+
+def _stream(device):
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _launch(what, device, *args):
     fn = getattr(lib(), what)
     if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        rc = fn(*args, _stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    check(rc, what)
+            rc = fn(*args, _stream(device))
+    if rc:
+        check(rc, what)
 
 
 def _check_rows(x):
@@ -157,8 +156,6 @@ def _check_rows(x):
 
 def _row_outputs(shape, device, out, scale):
     """``(q, q stride, scale)``: the destinations given, or new ones."""
-    import torch
-
     if out is None:
         out, stride = torch.empty(shape, dtype=torch.int8, device=device), shape[-1]
     else:
@@ -171,8 +168,6 @@ def _row_outputs(shape, device, out, scale):
 
 
 def _check_scale_out(scale, shape, device):
-    import torch
-
     if (scale.dtype != torch.float32 or tuple(scale.shape) != tuple(shape) or scale.device != device
             or not scale.is_contiguous() or scale.requires_grad):
         raise ValueError(f"scale must be a contiguous fp32 tensor of shape {list(shape)} on {device}")
@@ -223,8 +218,6 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_
 
     ``q`` is the integer nearest to ``127 h weight / max|h weight|`` (ties to even, decided exactly): the norm's factor
     cancels and only enters the scale.  Sums of squares are held in 64 bits."""
-    import torch
-
     code = _float_code(x, "x")
     _check_rows(x)
     width = x.shape[-1]
@@ -265,8 +258,6 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_
 
 
 def _check_quantized(q, scale, name):
-    import torch
-
     if q.dtype != torch.int8:
         raise TypeError(f"{name} must be an int8 tensor")
     if scale.dtype != torch.float32:
@@ -277,8 +268,6 @@ def _check_quantized(q, scale, name):
 
 def dequantize_int8(q, scale, dtype=None, out=None):
     """``q * scale`` of 8-bit rows ``q [..., K]`` with ``scale [...]``, in ``dtype`` (default fp16, or out's)."""
-    import torch
-
     _check_quantized(q, scale, "q")
     if not 1 <= q.shape[-1] <= MAX_WIDTH:
         raise ValueError(f"q must have a last axis of 1 to {MAX_WIDTH} values")
@@ -311,9 +300,8 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
     residual              ``[..., N]`` in ``dtype``, or None; ``out`` may be the residual itself
 
     Sums are int32 and exact for K up to 131071; scales, bias and residual are applied in fp32 and the result is rounded
-    once.  Rows that start at multiples of 16 bytes (K, or the row stride, a multiple of 16) are read fastest."""
-    import torch
-
+    once.  Operands whose rows start at multiples of 16 bytes (K and the row strides multiples of 16) are read as they are;
+    others are read more slowly or, in a large product, first copied to such rows in a workspace of the call."""
     _check_quantized(x, x_scale, "x")
     _check_quantized(weight, weight_scale, "weight")
     if weight.dim() != 2:
@@ -347,7 +335,13 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
         _check_apart((("out", out, (residual,)),), (x, x_scale, weight, weight_scale, bias, residual))
     tokens = x_scale.numel()
     if tokens and n:
-        _launch("tca_int8_linear_launch", device, x.data_ptr(), x_scale.data_ptr(), weight.data_ptr(),
-                weight_scale.data_ptr(), None if bias is None else bias.data_ptr(), r_ptr, out.data_ptr(), code, tokens,
-                n, k, x_stride, w_stride, r_stride, out_stride)
+        x_ptr, w_ptr = x.data_ptr(), weight.data_ptr()
+        workspace = None
+        if (x_ptr | w_ptr | x_stride | w_stride | k) & 15:
+            size = lib().tca_int8_linear_workspace_bytes(x_ptr, w_ptr, tokens, n, k, x_stride, w_stride)
+            if size:  # of this call: the allocator orders its reuse, also inside a graph's own pool
+                workspace = torch.empty(size, dtype=torch.int8, device=device)
+        _launch("tca_int8_linear_launch", device, x_ptr, x_scale.data_ptr(), w_ptr, weight_scale.data_ptr(),
+                None if bias is None else bias.data_ptr(), r_ptr, out.data_ptr(), code, tokens, n, k, x_stride,
+                w_stride, r_stride, out_stride, None if workspace is None else workspace.data_ptr())
     return out
