@@ -14,6 +14,64 @@ F32 = 2.0 ** -24  # half a step of fp32, relative
 TYPES = [torch.float16, torch.bfloat16, torch.float32]
 
 
+class _NoPlain:
+    """Stands in for the extension that takes plain calls: every call goes the general way."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def test_plain_and_general_calls_agree(monkeypatch):
+    """Contiguous operands are taken by the extension, everything else by the Python path: the same results."""
+    x, r = (_values(21, 96, torch.bfloat16, s).cuda() for s in (1, 2))
+    n = _values(1, 96, torch.bfloat16, 3)[0].cuda()
+    w, ws = _int8(40, 96).cuda(), torch.rand(40).cuda()
+    wu, wus = _int8(50, 97).cuda(), torch.rand(50).cuda()
+    b = torch.randn(40, device="cuda").bfloat16()
+
+    def calls():
+        q, s = int8.quantize_int8(x.reshape(3, 7, 96))
+        qu, su = int8.quantize_int8(_values(900, 97, torch.float32, 4).cuda())
+        yield from (q, s, qu, su)
+        yield from int8.silu_mul_int8(x)
+        yield from int8.rms_norm_int8(x, n, eps=1e-5)
+        yield from int8.rms_norm_int8(x, n.float(), residual=r)
+        yield from int8.rms_norm_int8(x[0], n, residual=r[0], eps=1)
+        for dtype in (None, *TYPES):
+            yield int8.dequantize_int8(q, s, dtype=dtype)
+            yield int8.linear_int8(q, s, w, ws, dtype=dtype)
+        yield int8.linear_int8(q, s, w, ws, bias=b, residual=torch.ones_like(x[:, :40]).reshape(3, 7, 40), dtype=b.dtype)
+        yield int8.linear_int8(qu, su, wu, wus)
+
+    plain = list(calls())
+    monkeypatch.setattr(int8, "_plain", _NoPlain())
+    general = list(calls())
+    assert len(plain) == len(general)
+    for p, g in zip(plain, general):
+        assert p.dtype == g.dtype and p.shape == g.shape and p.is_contiguous() and torch.equal(p, g)
+
+
+def test_plain_calls_are_taken_by_the_extension():
+    from triton_client_amd import _native
+
+    ops = _native.torch_ops()
+    x = _values(3, 32, torch.float16).cuda()
+    q, s = ops.quantize(x, False)
+    assert ops.dequantize(q, s, 1).dtype == torch.float16 and len(ops.quantize(x, True)) == 2
+    assert len(ops.rms_norm(x, x[0], None, 1e-6)) == 2 and len(ops.rms_norm(x, x[0], x, 1e-6)) == 3
+    assert ops.linear(q, s, q, s, None, None, 0).shape == (3, 3)
+    # not plain: left to the general path
+    assert ops.quantize(x.t(), False) is None and ops.quantize(x.cpu(), False) is None
+    assert ops.quantize(x.int(), False) is None and ops.quantize(x.clone().requires_grad_(), False) is None
+    assert ops.quantize(x[:, :31].contiguous(), True) is None and ops.quantize(None, False) is None
+    assert ops.rms_norm(x, x[0, :4], None, 1e-6) is None and ops.rms_norm(x, x[0], None, 0.0) is None
+    assert ops.rms_norm(x, x[0], x.float(), 1e-6) is None and ops.rms_norm(x, x[0], None, "1") is None
+    assert ops.dequantize(q, s[:2], 1) is None and ops.dequantize(x, s, 1) is None
+    assert ops.linear(q, s, q[:, :16].contiguous(), s, None, None, 0) is None
+    assert ops.linear(q, s, q, s, x[0, :3].contiguous(), None, 0) is None
+    assert ops.linear(q, s, q, s, None, x, 0) is None
+
+
 def _values(rows, width, dtype, seed=0, spread=1.0):
     g = torch.Generator().manual_seed(seed)
     x = torch.randn(rows, width, generator=g) * torch.exp(torch.randn(rows, 1, generator=g)) * spread

@@ -10,6 +10,7 @@ Targets
 -------
 core   : libtca_core.so      (g++   – system shm, codec, base64, image decoding C ABI)
 pyext  : _tca_pyext*.so      (g++   – CPython BYTES pack/unpack, native gRPC serving front)
+torch  : _tca_torch*.so       (g++   – the 8-bit operators' calls on torch tensors; where torch is installed)
 hip    : libtca_hip.so       (hipcc – hipshm + CDNA4 kernels)
 cpp    : build/libtcaclient.{a,so}, C++ examples, tests and the perf driver
 all    : everything above (default)
@@ -85,6 +86,26 @@ def build_pyext(force=False):
     return out
 
 
+def build_torch(force=False):
+    """``_tca_torch``: needs torch's headers, so it is built where torch is installed (client-only hosts go without)."""
+    import importlib.util
+
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return None
+    home = Path(list(spec.submodule_search_locations)[0])
+    out = LIBDIR / f"_tca_torch{sysconfig.get_config_var('EXT_SUFFIX')}"
+    src = CSRC / "capi" / "torch_ops.cc"
+    if force or _stale(out, [src, home / "version.py"]):
+        LIBDIR.mkdir(exist_ok=True)
+        _compile_atomic(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+                         "-isystem", home / "include", "-isystem",
+                         home / "include" / "torch" / "csrc" / "api" / "include", "-isystem", ROCM / "include",
+                         "-isystem", sysconfig.get_paths()["include"], "-o", out, src, f"-L{home / 'lib'}",
+                         "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"], out)
+    return out
+
+
 def hip_sources():
     return sorted((CSRC / "hip").glob("*.hip")) + sorted((CSRC / "hip").glob("*.cc"))
 
@@ -135,7 +156,7 @@ def build_cpp(force=False):
     return BUILD
 
 
-TARGETS = {"core": build_core, "pyext": build_pyext, "hip": build_hip, "cpp": build_cpp}
+TARGETS = {"core": build_core, "pyext": build_pyext, "torch": build_torch, "hip": build_hip, "cpp": build_cpp}
 
 
 def build(targets=None, force=False):

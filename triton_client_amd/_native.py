@@ -156,6 +156,30 @@ def pyext():
     return _tca_pyext
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The ``_tca_torch`` CPython extension (built on demand), with the launchers of libtca_hip.so handed to it."""
+    global _torch_ops
+    if _torch_ops is None:
+        import torch  # noqa: F401 - its libraries have to be there before the extension's symbols are bound
+
+        try:
+            from ._lib import _tca_torch
+        except ImportError:
+            from . import _build
+
+            _build.build_torch()
+            from ._lib import _tca_torch
+        lib = hip()
+        _tca_torch.use(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "tca_int8_quantize_launch", "tca_int8_rms_norm_launch", "tca_int8_dequantize_launch",
+            "tca_int8_linear_launch", "tca_int8_linear_workspace_bytes")))
+        _torch_ops = _tca_torch
+    return _torch_ops
+
+
 def pyext_available():
     try:
         from ._lib import _tca_pyext  # noqa: F401

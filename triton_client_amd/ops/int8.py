@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import torch
 
+from .. import _native
 from ._device import check, lib
 
 # 128 * 128 * k has to stay below 2^31
@@ -40,11 +41,14 @@ MAX_WIDTH = 1 << 29
 _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _float_code(t, name):
-    code = _CODES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name} must be an fp16, bf16 or fp32 tensor")
-    return code
+# the extension that takes the plain case of a call (contiguous operands, new results) without the checks below
+_plain = None
+
+
+def _load_plain():
+    global _plain
+    _plain = _native.torch_ops()
+    return _plain
 
 
 def _output_code(dtype):
@@ -54,21 +58,25 @@ def _output_code(dtype):
     return code
 
 
-def _refuse_gradients(*operands):
-    for t in operands:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("8-bit operators have no gradient: detach the operands or call under torch.no_grad()")
-
-
-def _same_device(first, *others):
-    """The common CUDA device of the operands."""
-    device = first.device
-    if device.type != "cuda":
-        raise ValueError("the operands must be CUDA tensors")
+def _check_operands(first, others):
+    """Index of the operands' common CUDA device; no operand may require a gradient while gradients are recorded."""
+    device = first.get_device()
+    if first.requires_grad:
+        _refuse_gradient()
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError("the operands must be on one device")
+        if t is not None:
+            if t.requires_grad:
+                _refuse_gradient()
+            if t.get_device() != device:
+                raise ValueError("the operands must be on one device")
+    if device < 0:
+        raise ValueError("the operands must be CUDA tensors")
     return device
+
+
+def _refuse_gradient():
+    if torch.is_grad_enabled():
+        raise ValueError("8-bit operators have no gradient: detach the operands or call under torch.no_grad()")
 
 
 def _rows(t):
@@ -130,40 +138,35 @@ def _check_apart(outputs, inputs):
                 raise ValueError(f"{name} overlaps {other}")
 
 
-# the handle alone, where torch gives it: an object around it costs more than the checks of a call
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+def _raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _stream(device):
-    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+# the handle alone, where torch gives it: an object around it costs as much as a third of a call's checks
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 def _launch(what, device, *args):
     fn = getattr(lib(), what)
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, _stream(device))
+    if torch.cuda.current_device() == device:
+        rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _stream(device))
+            rc = fn(*args, _raw_stream(device))
     if rc:
         check(rc, what)
 
 
-def _check_rows(x):
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
-        raise ValueError(f"x must have a last axis of 1 to {MAX_WIDTH} values")
-
-
-def _row_outputs(shape, device, out, scale):
+def _row_outputs(x, shape, out, scale):
     """``(q, q stride, scale)``: the destinations given, or new ones."""
     if out is None:
-        out, stride = torch.empty(shape, dtype=torch.int8, device=device), shape[-1]
+        out, stride = torch.empty(shape, dtype=torch.int8, device=x.device), shape[-1]
     else:
-        stride = _out_rows(out, shape, torch.int8, device, "out")
+        stride = _out_rows(out, shape, torch.int8, x.device, "out")
     if scale is None:
-        scale = torch.empty(shape[:-1], dtype=torch.float32, device=device)
+        scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
     else:
-        _check_scale_out(scale, shape[:-1], device)
+        _check_scale_out(scale, shape[:-1], x.device)
     return out, stride, scale
 
 
@@ -173,18 +176,26 @@ def _check_scale_out(scale, shape, device):
         raise ValueError(f"scale must be a contiguous fp32 tensor of shape {list(shape)} on {device}")
 
 
-def _quantize(x, width, gated, out, scale):
-    code = _float_code(x, "x")
-    _refuse_gradients(x)
-    device = _same_device(x, out, scale)
+def _quantize(x, gated, out, scale):
+    code = _CODES.get(x.dtype)
+    if code is None:
+        raise TypeError("x must be an fp16, bf16 or fp32 tensor")
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"x must have a last axis of 1 to {MAX_WIDTH} values")
+    if gated:
+        if shape[-1] % 2:
+            raise ValueError("the last axis of x must hold two halves of equal size")
+        shape = (*shape[:-1], shape[-1] // 2)
+    device = _check_operands(x, (out, scale))
     x, x_stride = _rows(x)
-    q, q_stride, s = _row_outputs((*x.shape[:-1], width), device, out, scale)
+    q, q_stride, s = _row_outputs(x, shape, out, scale)
     if out is not None or scale is not None:
         _check_apart((("out", out, ()), ("scale", scale, ())), (x,))
     rows = s.numel()
     if rows:
-        _launch("tca_int8_quantize_launch", device, x.data_ptr(), q.data_ptr(), s.data_ptr(), code, gated, rows, width,
-                x_stride, q_stride)
+        _launch("tca_int8_quantize_launch", device, x.data_ptr(), q.data_ptr(), s.data_ptr(), code, gated, rows,
+                shape[-1], x_stride, q_stride)
     return q, s
 
 
@@ -192,18 +203,22 @@ def quantize_int8(x, out=None, scale=None):
     """``(q int8 [..., K], scale fp32 [...])`` of ``x [..., K]``: with ``m`` the largest magnitude of a row, ``q`` is the
     integer nearest to ``127 x / m`` (ties to even, decided exactly) and ``scale = m / 127`` (one step less where
     ``127 * scale`` would leave fp32's range).  A row of zeros has the scale 0.  ``out`` and ``scale`` may be destinations of the results' shapes."""
-    _check_rows(x)
-    return _quantize(x, x.shape[-1], 0, out, scale)
+    if out is None and scale is None:
+        made = (_plain or _load_plain()).quantize(x, False)
+        if made is not None:
+            return made
+    return _quantize(x, 0, out, scale)
 
 
 def silu_mul_int8(x, out=None, scale=None):
     """8-bit rows ``(q [..., K], scale [...])``, as of :func:`quantize_int8`, of ``silu(gate) * up`` for
     ``x [..., 2 K]`` with the gate in the first half of the last axis and the other factor in the second.  The product
     is taken in fp32."""
-    _check_rows(x)
-    if x.shape[-1] % 2:
-        raise ValueError("the last axis of x must hold two halves of equal size")
-    return _quantize(x, x.shape[-1] // 2, 1, out, scale)
+    if out is None and scale is None:
+        made = (_plain or _load_plain()).quantize(x, True)
+        if made is not None:
+            return made
+    return _quantize(x, 1, out, scale)
 
 
 def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_out=None):
@@ -218,34 +233,40 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_
 
     ``q`` is the integer nearest to ``127 h weight / max|h weight|`` (ties to even, decided exactly): the norm's factor
     cancels and only enters the scale.  Sums of squares are held in 64 bits."""
-    code = _float_code(x, "x")
-    _check_rows(x)
-    width = x.shape[-1]
+    if out is None and scale is None and sum_out is None:
+        made = (_plain or _load_plain()).rms_norm(x, weight, residual, eps)
+        if made is not None:
+            return made
+    dtype = x.dtype
+    code = _CODES.get(dtype)
+    if code is None:
+        raise TypeError("x must be an fp16, bf16 or fp32 tensor")
+    shape = x.shape
+    if not shape or not 1 <= shape[-1] <= MAX_WIDTH:
+        raise ValueError(f"x must have a last axis of 1 to {MAX_WIDTH} values")
+    width = shape[-1]
     weight_f32 = weight.dtype == torch.float32
-    if not weight_f32 and weight.dtype != x.dtype:
+    if not weight_f32 and weight.dtype != dtype:
         raise TypeError("weight must have x's type or be fp32")
-    if tuple(weight.shape) != (width,) or not weight.is_contiguous():
+    if weight.dim() != 1 or weight.shape[0] != width or not weight.is_contiguous():
         raise ValueError(f"weight must be a contiguous vector of {width} values")
-    eps = float(eps)
     if not 0.0 < eps < float("inf"):
         raise ValueError("eps must be a positive number")
     if residual is None:
         if sum_out is not None:
             raise ValueError("sum_out needs a residual")
-    elif residual.dtype != x.dtype or residual.shape != x.shape:
+    elif residual.dtype != dtype or residual.shape != shape:
         raise ValueError("residual must have x's type and shape")
-    _refuse_gradients(x, weight, residual)
-    device = _same_device(x, weight, residual, out, scale, sum_out)
-    shape = x.shape
+    device = _check_operands(x, (weight, residual, out, scale, sum_out))
     x, x_stride = _rows(x)
-    q, q_stride, s = _row_outputs(tuple(shape), device, out, scale)
+    q, q_stride, s = _row_outputs(x, shape, out, scale)
     summed, r_ptr, sum_ptr, r_stride, sum_stride = None, None, None, 0, 0
     if residual is not None:
         residual, r_stride = _rows(residual)
         if sum_out is None:
-            summed, sum_stride = torch.empty(shape, dtype=x.dtype, device=device), width
+            summed, sum_stride = torch.empty(shape, dtype=dtype, device=x.device), width
         else:
-            summed, sum_stride = sum_out, _out_rows(sum_out, shape, x.dtype, device, "sum_out")
+            summed, sum_stride = sum_out, _out_rows(sum_out, shape, dtype, x.device, "sum_out")
         r_ptr, sum_ptr = residual.data_ptr(), summed.data_ptr()
     if out is not None or scale is not None or sum_out is not None:
         _check_apart((("out", out, ()), ("scale", scale, ()), ("sum_out", sum_out, (x, residual))),
@@ -257,32 +278,37 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_
     return (q, s) if residual is None else (q, s, summed)
 
 
-def _check_quantized(q, scale, name):
+def _check_quantized(q, scale, name, scale_name):
     if q.dtype != torch.int8:
         raise TypeError(f"{name} must be an int8 tensor")
     if scale.dtype != torch.float32:
-        raise TypeError(f"{name}_scale must be an fp32 tensor" if name != "q" else "scale must be an fp32 tensor")
-    if q.dim() < 1 or scale.shape != q.shape[:-1]:
+        raise TypeError(f"{scale_name} must be an fp32 tensor")
+    shape = q.shape
+    if not shape or scale.shape != shape[:-1]:
         raise ValueError(f"{name} [..., K] needs a scale for each row, of shape [...]")
+    return shape
 
 
 def dequantize_int8(q, scale, dtype=None, out=None):
     """``q * scale`` of 8-bit rows ``q [..., K]`` with ``scale [...]``, in ``dtype`` (default fp16, or out's)."""
-    _check_quantized(q, scale, "q")
-    if not 1 <= q.shape[-1] <= MAX_WIDTH:
+    if out is None:
+        code = _output_code(torch.float16 if dtype is None else dtype)
+        made = (_plain or _load_plain()).dequantize(q, scale, code)
+        if made is not None:
+            return made
+    shape = _check_quantized(q, scale, "q", "scale")
+    if not 1 <= shape[-1] <= MAX_WIDTH:
         raise ValueError(f"q must have a last axis of 1 to {MAX_WIDTH} values")
     if dtype is None:
         dtype = torch.float16 if out is None else out.dtype
     code = _output_code(dtype)
-    _refuse_gradients(scale)
-    device = _same_device(q, scale, out)
-    shape = q.shape
+    device = _check_operands(scale, (q, out))
     q, q_stride = _rows(q)
     scale = scale.contiguous()
     if out is None:
-        out, out_stride = torch.empty(shape, dtype=dtype, device=device), shape[-1]
+        out, out_stride = torch.empty(shape, dtype=dtype, device=q.device), shape[-1]
     else:
-        out_stride = _out_rows(out, shape, dtype, device, "out")
+        out_stride = _out_rows(out, shape, dtype, q.device, "out")
         _check_apart((("out", out, ()),), (q, scale))
     rows = scale.numel()
     if rows:
@@ -302,25 +328,29 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
     Sums are int32 and exact for K up to 131071; scales, bias and residual are applied in fp32 and the result is rounded
     once.  Operands whose rows start at multiples of 16 bytes (K and the row strides multiples of 16) are read as they are;
     others are read more slowly or, in a large product, first copied to such rows in a workspace of the call."""
-    _check_quantized(x, x_scale, "x")
-    _check_quantized(weight, weight_scale, "weight")
-    if weight.dim() != 2:
+    if out is None:
+        code = _output_code(torch.float16 if dtype is None else dtype)
+        made = (_plain or _load_plain()).linear(x, x_scale, weight, weight_scale, bias, residual, code)
+        if made is not None:
+            return made
+    shape = _check_quantized(x, x_scale, "x", "x_scale")
+    w_shape = _check_quantized(weight, weight_scale, "weight", "weight_scale")
+    if len(w_shape) != 2:
         raise ValueError("weight must be an [N, K] matrix")
-    n, k = weight.shape
-    if x.shape[-1] != k:
-        raise ValueError(f"x has rows of {x.shape[-1]} integers, weight of {k}")
+    n, k = w_shape
+    if shape[-1] != k:
+        raise ValueError(f"x has rows of {shape[-1]} integers, weight of {k}")
     if not 1 <= k <= MAX_K:
         raise ValueError(f"K must be 1 to {MAX_K}: the int32 sums hold no more")
     if dtype is None:
         dtype = torch.float16 if out is None else out.dtype
     code = _output_code(dtype)
-    shape = (*x.shape[:-1], n)
+    shape = (*shape[:-1], n)
     if bias is not None and (bias.dtype != dtype or tuple(bias.shape) != (n,) or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous {dtype} vector of {n} values")
     if residual is not None and (residual.dtype != dtype or tuple(residual.shape) != shape):
         raise ValueError(f"residual must be a {dtype} tensor of shape {list(shape)}")
-    _refuse_gradients(x_scale, weight_scale, bias, residual)
-    device = _same_device(x, x_scale, weight, weight_scale, bias, residual, out)
+    device = _check_operands(x_scale, (x, weight, weight_scale, bias, residual, out))
     x, x_stride = _rows(x)
     weight, w_stride = _rows(weight)
     x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
@@ -329,9 +359,9 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
         residual, r_stride = _rows(residual)
         r_ptr = residual.data_ptr()
     if out is None:
-        out, out_stride = torch.empty(shape, dtype=dtype, device=device), n
+        out, out_stride = torch.empty(shape, dtype=dtype, device=x.device), n
     else:
-        out_stride = _out_rows(out, shape, dtype, device, "out")
+        out_stride = _out_rows(out, shape, dtype, x.device, "out")
         _check_apart((("out", out, (residual,)),), (x, x_scale, weight, weight_scale, bias, residual))
     tokens = x_scale.numel()
     if tokens and n:
@@ -340,7 +370,7 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
         if (x_ptr | w_ptr | x_stride | w_stride | k) & 15:
             size = lib().tca_int8_linear_workspace_bytes(x_ptr, w_ptr, tokens, n, k, x_stride, w_stride)
             if size:  # of this call: the allocator orders its reuse, also inside a graph's own pool
-                workspace = torch.empty(size, dtype=torch.int8, device=device)
+                workspace = torch.empty(size, dtype=torch.int8, device=x.device)
         _launch("tca_int8_linear_launch", device, x_ptr, x_scale.data_ptr(), w_ptr, weight_scale.data_ptr(),
                 None if bias is None else bias.data_ptr(), r_ptr, out.data_ptr(), code, tokens, n, k, x_stride,
                 w_stride, r_stride, out_stride, None if workspace is None else workspace.data_ptr())
