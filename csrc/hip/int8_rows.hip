@@ -38,21 +38,11 @@ struct Bf16 {
 
 // ---- chunks of eight values; addresses need no alignment beyond the element's own --------------------------------
 
-__device__ __forceinline__ void Unpack(const float* p, float (&v)[kVec]) {
-  __builtin_memcpy(v, p, sizeof(v));
-}
-__device__ __forceinline__ void Unpack(const _Float16* p, float (&v)[kVec]) {
-  half8 h;
-  __builtin_memcpy(&h, p, sizeof(h));
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] = static_cast<float>(h[i]);
-}
-__device__ __forceinline__ void Unpack(const Bf16* p, float (&v)[kVec]) {
-  ushort8 h;
-  __builtin_memcpy(&h, p, sizeof(h));
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] = __uint_as_float(static_cast<unsigned>(h[i]) << 16);
-}
+template <typename T>
+struct Chunk {  // as it lies in memory
+  static constexpr int kWords = 2 * sizeof(T);
+  unsigned raw[kWords];
+};
 
 __device__ __forceinline__ float ToFloat(float v) { return v; }
 __device__ __forceinline__ float ToFloat(_Float16 v) { return static_cast<float>(v); }
@@ -65,14 +55,48 @@ template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
   return Bf16{__builtin_bit_cast(unsigned short, static_cast<__bf16>(v))};  // nearest, ties to even, NaN kept
 }
 
-template <typename T>
-__device__ __forceinline__ void LoadChunk(const T* row, int first, int width, float (&v)[kVec]) {
-  if (first + kVec <= width) {
-    Unpack(row + first, v);
+// The chunk at `first`.  Where the row ends inside it, its last eight values instead; behind the row's end, values that
+// are not used.  No branch: all requests of a thread are on their way before it waits for one.  Rows shorter than a
+// chunk (kShort) are read one by one.
+template <bool kShort, typename T>
+__device__ __forceinline__ Chunk<T> Request(const T* row, int first, int width) {
+  Chunk<T> c;
+  if constexpr (!kShort) {
+    __builtin_memcpy(&c, row + min(first, width - kVec), sizeof(c));
   } else {
+    T t[kVec];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = first + i < width ? ToFloat(row[first + i]) : 0.f;
+    for (int i = 0; i < kVec; ++i) t[i] = i < width ? row[i] : T{};
+    __builtin_memcpy(&c, t, sizeof(c));
   }
+  return c;
+}
+
+// Its values, zeros behind the row's end
+template <bool kShort, typename T>
+__device__ __forceinline__ void Values(Chunk<T> c, int first, int width, float (&v)[kVec]) {
+  constexpr int kWords = Chunk<T>::kWords;
+  const int past = first + kVec - width;  // values that belong to the chunk before this one
+  if (!kShort && past > 0) {              // they are moved out
+#pragma unroll
+    for (int step = 4; step >= 1; step /= 2) {
+      if (past & step) {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+          if constexpr (sizeof(T) == 2) {
+            if (step == 1) c.raw[i] = c.raw[i] >> 16 | (i + 1 < kWords ? c.raw[i + 1] << 16 : 0u);
+            else c.raw[i] = i + step / 2 < kWords ? c.raw[i + step / 2] : 0u;
+          } else {
+            c.raw[i] = i + step < kWords ? c.raw[i + step] : 0u;
+          }
+        }
+      }
+    }
+  }
+  T t[kVec];
+  __builtin_memcpy(t, &c, sizeof(t));
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) v[i] = ToFloat(t[i]);
 }
 
 template <typename T>
@@ -106,29 +130,66 @@ struct RowArgs {
   double eps;
 };
 
+// g / (1 + exp(-g)), within 7 half steps of fp32 (2^-24).  With z = exp(-|g|) <= 1 it is g / (1 + z) or g z / (1 + z), in
+// which nothing overflows.  z = 2^n 2^f for the integer n nearest to -|g| log2 e: f is that product less n in fused steps
+// with log2 e in two parts, 2^f comes from the unit; the quotient from the unit's reciprocal and one correction.  16
+// instructions where the library's exp and division take about 40, and the kernel was bound by them.
+__device__ __forceinline__ float Silu(float g) {
+  constexpr float kLog2E = 0x1.715476p+0f, kLog2ELow = 0x1.4ae0cp-26f;
+  const float a = -fminf(fabsf(g), 200.f);  // exp(-200) is 0 in fp32
+  const float n = rintf(a * kLog2E);
+  const float f = fmaf(a, kLog2ELow, fmaf(a, kLog2E, -n));
+  const float z = ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n));
+  const float d = 1.f + z, r = __builtin_amdgcn_rcpf(d);
+  const float over = g < 0.f ? g * z : g;
+  const float y = over * r;
+  return fmaf(fmaf(-y, d, over), r, y);
+}
+
+// What a chunk of p is made from: x; the other factor, or the residual; the weight, of type W
+template <typename T, typename W>
+struct Inputs {
+  Chunk<T> x, second;
+  Chunk<W> weight;
+};
+
+template <typename T>
+__device__ __forceinline__ const T* Row(const void* p, long long row, long long stride) {
+  return static_cast<const T*>(p) + row * stride;
+}
+
+template <typename T, typename W, int kMode, bool kShort>
+__device__ __forceinline__ Inputs<T, W> RequestInputs(const RowArgs& a, long long row, int first) {
+  Inputs<T, W> in;
+  const T* x = Row<T>(a.x, row, a.x_stride);
+  in.x = Request<kShort>(x, first, a.width);
+  if constexpr (kMode == kGate) in.second = Request<kShort>(x + a.width, first, a.width);
+  if constexpr (kMode == kNormResidual) in.second = Request<kShort>(Row<T>(a.residual, row, a.residual_stride), first, a.width);
+  if constexpr (kMode == kNorm || kMode == kNormResidual) in.weight = Request<kShort>(static_cast<const W*>(a.weight), first, a.width);
+  return in;
+}
+
 // p of chunk `first`; kNormResidual also writes the sum, rounded to T, and normalises the rounded one
-template <typename T, int kMode>
-__device__ __forceinline__ void RowChunk(const RowArgs& a, long long row, int first, float (&p)[kVec], double& squares,
-                                         bool write_sum) {
-  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
-  LoadChunk(x, first, a.width, p);
+template <typename T, typename W, int kMode, bool kShort>
+__device__ __forceinline__ void RowChunk(const RowArgs& a, long long row, int first, const Inputs<T, W>& in,
+                                         float (&p)[kVec], double& squares) {
+  Values<kShort>(in.x, first, a.width, p);
   if constexpr (kMode == kGate) {
     float up[kVec];
-    LoadChunk(x + a.width, first, a.width, up);
+    Values<kShort>(in.second, first, a.width, up);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) p[i] = p[i] / (1.f + expf(-p[i])) * up[i];
+    for (int i = 0; i < kVec; ++i) p[i] = Silu(p[i]) * up[i];
   }
   if constexpr (kMode == kNormResidual) {
     float r[kVec];
-    LoadChunk(static_cast<const T*>(a.residual) + row * a.residual_stride, first, a.width, r);
+    Values<kShort>(in.second, first, a.width, r);
 #pragma unroll
     for (int i = 0; i < kVec; ++i) p[i] = ToFloat(FromFloat<T>(p[i] + r[i]));
-    if (write_sum) StoreChunk(static_cast<T*>(a.sum) + row * a.sum_stride, first, a.width, p);
+    StoreChunk(static_cast<T*>(a.sum) + row * a.sum_stride, first, a.width, p);
   }
   if constexpr (kMode == kNorm || kMode == kNormResidual) {
     float w[kVec];
-    if (a.weight_f32) LoadChunk(static_cast<const float*>(a.weight), first, a.width, w);
-    else LoadChunk(static_cast<const T*>(a.weight), first, a.width, w);
+    Values<kShort>(in.weight, first, a.width, w);
     // squares in 64 bits: they hold for every value of the 32-bit range, where 32-bit squares overflow from 2^64
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
@@ -170,10 +231,12 @@ __device__ __forceinline__ uint64_t Levels(const float (&p)[kVec], float top, fl
 #pragma unroll
     for (int i = 0; i < kVec; ++i) level[i] = static_cast<unsigned>(ExactLevel(p[i], top));
   }
-  uint64_t packed = 0;
+  unsigned half[2];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) packed |= static_cast<uint64_t>(level[i] & 0xffu) << (8 * i);
-  return packed;
+  for (int h = 0; h < 2; ++h)  // the low bytes of four
+    half[h] = __builtin_amdgcn_perm(level[4 * h + 1], level[4 * h], 0x0c0c0400u) |
+              __builtin_amdgcn_perm(level[4 * h + 3], level[4 * h + 2], 0x04000c0cu);
+  return half[0] | static_cast<uint64_t>(half[1]) << 32;
 }
 
 __device__ __forceinline__ void StoreLevels(int8_t* row, int first, int width, uint64_t packed) {
@@ -181,35 +244,67 @@ __device__ __forceinline__ void StoreLevels(int8_t* row, int first, int width, u
     __builtin_memcpy(row + first, &packed, sizeof(packed));
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i)
+    for (int i = 0; i < kVec - 1; ++i)
       if (first + i < width) row[first + i] = static_cast<int8_t>(packed >> (8 * i));
   }
 }
 
-// the row's maximum and sum of squares over all threads of the row
-template <bool kNeedSum, bool kOneWave>
-__device__ __forceinline__ void ReduceRow(unsigned& top, double& squares) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) {
-    top = max(top, static_cast<unsigned>(__shfl_xor(static_cast<int>(top), d, 64)));
-    if constexpr (kNeedSum) squares += __shfl_xor(squares, d, 64);
+// v of the lanes that step s of a reduction over the wave puts together: within rows of 16 lanes through the data path's
+// own permutations, then by exchanging rows.  The same pair in the same order, or its mirror image, in both lanes.
+template <int kStep>
+__device__ __forceinline__ void Pair(unsigned v, unsigned& first, unsigned& second) {
+  if constexpr (kStep < 4) {
+    constexpr int kPermutation[] = {0xB1, 0x4E, 0x141, 0x140};  // lanes 1 0 3 2, 2 3 0 1, half rows and rows mirrored
+    first = v;
+    second = __builtin_amdgcn_update_dpp(0, v, kPermutation[kStep], 0xf, 0xf, true);
+  } else if constexpr (kStep == 4) {
+    const auto swapped = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    first = swapped[0];
+    second = swapped[1];
+  } else {
+    const auto swapped = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    first = swapped[0];
+    second = swapped[1];
   }
-  if constexpr (!kOneWave) {
-    __shared__ unsigned tops[16];
-    __shared__ double sums[16];
-    const int waves = blockDim.x >> 6;
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-      tops[wave] = top;
-      if constexpr (kNeedSum) sums[wave] = squares;
+}
+
+template <bool kNeedSum, int kSteps = 6, int kStep = 0>
+__device__ __forceinline__ void ReduceWave(unsigned& top, double& squares) {  // over 2^kSteps neighbouring lanes
+  if constexpr (kStep < kSteps) {
+    unsigned first, second;
+    Pair<kStep>(top, first, second);
+    top = max(first, second);
+    if constexpr (kNeedSum) {
+      const uint64_t bits = __builtin_bit_cast(uint64_t, squares);
+      unsigned low[2], high[2];
+      Pair<kStep>(static_cast<unsigned>(bits), low[0], low[1]);
+      Pair<kStep>(static_cast<unsigned>(bits >> 32), high[0], high[1]);
+      squares = __builtin_bit_cast(double, low[0] | static_cast<uint64_t>(high[0]) << 32) +
+                __builtin_bit_cast(double, low[1] | static_cast<uint64_t>(high[1]) << 32);
     }
-    __syncthreads();
-    top = tops[0];
-    if constexpr (kNeedSum) squares = sums[0];
-    for (int i = 1; i < waves; ++i) {  // the same order in every thread
-      top = max(top, tops[i]);
-      if constexpr (kNeedSum) squares += sums[i];
-    }
+    ReduceWave<kNeedSum, kSteps, kStep + 1>(top, squares);
+  }
+}
+
+// the row's maximum and sum of squares over all threads of the row
+template <bool kNeedSum>
+__device__ __forceinline__ void ReduceRow(unsigned& top, double& squares) {
+  ReduceWave<kNeedSum>(top, squares);
+  const int waves = blockDim.x >> 6;
+  if (waves == 1) return;
+  __shared__ unsigned tops[16];
+  __shared__ double sums[16];
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    tops[wave] = top;
+    if constexpr (kNeedSum) sums[wave] = squares;
+  }
+  __syncthreads();
+  top = tops[0];
+  if constexpr (kNeedSum) squares = sums[0];
+  for (int i = 1; i < waves; ++i) {  // the same order in every thread
+    top = max(top, tops[i]);
+    if constexpr (kNeedSum) squares += sums[i];
   }
 }
 
@@ -227,29 +322,28 @@ __device__ __forceinline__ void StoreScale(const RowArgs& a, long long row, unsi
   }
 }
 
-// kChunks chunks per thread stay in registers.  kOneWave: a wavefront per row, four rows per block, no barrier;
-// otherwise a block per row.
-template <typename T, int kMode, int kChunks, bool kOneWave>
-__global__ __launch_bounds__(kOneWave ? 256 : 1024) void RowsKernel(RowArgs a) {
-  constexpr bool kNeedSum = kMode == kNorm || kMode == kNormResidual;
-  const int threads = kOneWave ? 64 : blockDim.x;
-  const int t = kOneWave ? (threadIdx.x & 63) : threadIdx.x;
-  const long long row = kOneWave ? a.first_row + static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 6)
-                                 : a.first_row + blockIdx.x;
-  if (kOneWave && row >= a.rows) return;
-  float p[kChunks][kVec];
-  unsigned top = 0;
-  double squares = 0.0;
+// p of kChunks chunks in registers, the maximum and the sum of this thread's
+template <typename T, typename W, int kMode, int kChunks, bool kShort>
+__device__ __forceinline__ void TakeRow(const RowArgs& a, long long row, int t, int threads, float (&p)[kChunks][kVec],
+                                        unsigned& top, double& squares) {
+  Inputs<T, W> in[kChunks];
+#pragma unroll
+  for (int c = 0; c < kChunks; ++c) in[c] = RequestInputs<T, W, kMode, kShort>(a, row, (c * threads + t) * kVec);
+  top = 0;
+  squares = 0.0;
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
     const int first = (c * threads + t) * kVec;
     if (first < a.width) {
-      RowChunk<T, kMode>(a, row, first, p[c], squares, true);
+      RowChunk<T, W, kMode, kShort>(a, row, first, in[c], p[c], squares);
       top = MaxBits(p[c], top);
     }
   }
-  ReduceRow<kNeedSum, kOneWave>(top, squares);
-  if (t == 0) StoreScale<kMode>(a, row, top, squares);
+}
+
+template <int kMode, int kChunks>
+__device__ __forceinline__ void GiveRow(const RowArgs& a, long long row, int t, int threads, const float (&p)[kChunks][kVec],
+                                        unsigned top, double squares) {
   const float largest = __uint_as_float(top);
   const bool live = top != 0 && top < kInfBits;  // the same in the whole row
   const float inverse = 127.f / largest;
@@ -259,22 +353,51 @@ __global__ __launch_bounds__(kOneWave ? 256 : 1024) void RowsKernel(RowArgs a) {
     const int first = (c * threads + t) * kVec;
     if (first < a.width) StoreLevels(q, first, a.width, live ? Levels(p[c], largest, inverse) : 0);
   }
+  if (t == 0) StoreScale<kMode>(a, row, top, squares);
+}
+
+// A block per row, kChunks chunks per thread.
+template <typename T, typename W, int kMode, int kChunks>
+__global__ __launch_bounds__(1024) void RowsKernel(RowArgs a) {
+  const long long row = a.first_row + blockIdx.x;
+  float p[kChunks][kVec];
+  unsigned top;
+  double squares;
+  TakeRow<T, W, kMode, kChunks, false>(a, row, threadIdx.x, blockDim.x, p, top, squares);
+  ReduceRow<kMode == kNorm || kMode == kNormResidual>(top, squares);
+  GiveRow<kMode>(a, row, threadIdx.x, blockDim.x, p, top, squares);
+}
+
+// Rows of at most 8, 16 or 32 chunks: 2^kSteps lanes per row, 256 threads per block.
+template <typename T, typename W, int kMode, int kSteps, bool kShort>
+__global__ __launch_bounds__(256) void NarrowRowsKernel(RowArgs a) {
+  constexpr int kLanes = 1 << kSteps;
+  const long long row = a.first_row + static_cast<long long>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  const int t = threadIdx.x % kLanes;
+  if (row >= a.rows) return;
+  float p[1][kVec];
+  unsigned top;
+  double squares;
+  TakeRow<T, W, kMode, 1, kShort>(a, row, t, kLanes, p, top, squares);
+  ReduceWave<kMode == kNorm || kMode == kNormResidual, kSteps>(top, squares);
+  GiveRow<kMode>(a, row, t, kLanes, p, top, squares);
 }
 
 // Rows that do not fit into a block's registers: the row is read twice, the second time mostly from L2.  The second
-// pass computes p anew from the inputs - except that a sum written over one of them is read back instead.
-template <typename T, int kMode>
+// pass computes p anew from the inputs; a sum, which may lie over one of them, is read back instead.
+template <typename T, typename W, int kMode>
 __global__ __launch_bounds__(1024) void LongRowsKernel(RowArgs a) {
   constexpr bool kNeedSum = kMode == kNorm || kMode == kNormResidual;
   const long long row = a.first_row + blockIdx.x;
   unsigned top = 0;
   double squares = 0.0;
   for (long long at = threadIdx.x; at * kVec < a.width; at += blockDim.x) {
+    const int first = static_cast<int>(at) * kVec;
     float p[kVec];
-    RowChunk<T, kMode>(a, row, static_cast<int>(at) * kVec, p, squares, true);
+    RowChunk<T, W, kMode, false>(a, row, first, RequestInputs<T, W, kMode, false>(a, row, first), p, squares);
     top = MaxBits(p, top);
   }
-  ReduceRow<kNeedSum, false>(top, squares);
+  ReduceRow<kNeedSum>(top, squares);
   if (threadIdx.x == 0) StoreScale<kMode>(a, row, top, squares);
   const float largest = __uint_as_float(top);
   const bool live = top != 0 && top < kInfBits;
@@ -290,7 +413,7 @@ __global__ __launch_bounds__(1024) void LongRowsKernel(RowArgs a) {
     const int first = static_cast<int>(at) * kVec;
     float p[kVec];
     double unused = 0.0;
-    RowChunk<T, kAgain>(again, row, first, p, unused, false);
+    RowChunk<T, W, kAgain, false>(again, row, first, RequestInputs<T, W, kAgain, false>(again, row, first), p, unused);
     StoreLevels(q, first, a.width, live ? Levels(p, largest, inverse) : 0);
   }
 }
@@ -330,34 +453,51 @@ int Status() {
 // A grid holds fewer than 2^32 threads: rows beyond that go to further launches.
 constexpr long long kMostRows = 1ll << 21;
 
-template <typename T, int kMode>
+// Few rows: as many threads as a row has chunks, every chunk's way from memory at the same time (8 rows of 8192 bf16: 5.0
+// us with one chunk per thread, 7.0 with four).  Many rows fill the CUs anyway, and four chunks per thread keep more bytes
+// on their way in fewer waves (16384 rows: 81 us with four, 135 with one).  Norms of fp32 rows hold three fp32 inputs per
+// value: two chunks are what the registers of 1024 threads hold.
+template <typename T, typename W, int kMode>
 void LaunchRows(RowArgs a, hipStream_t stream) {
+  constexpr bool kWide = sizeof(T) == 4 && (kMode == kNorm || kMode == kNormResidual);
   const int chunks = (a.width + kVec - 1) / kVec;
-  auto threads = [&](int per_thread) { return dim3(((chunks + per_thread - 1) / per_thread + 63) / 64 * 64); };
   const long long rows = a.rows;
+  const int most = kWide ? 2 : 4;
+  int per_thread = rows >= 2048 && chunks >= 512 ? most : 1;
+  while (per_thread < most && chunks > per_thread * 1024) per_thread *= 2;
+  const dim3 threads(((chunks + per_thread - 1) / per_thread + 63) / 64 * 64);
   for (; a.first_row < rows; a.first_row += kMostRows) {
-    a.rows = rows - a.first_row < kMostRows ? rows : a.first_row + kMostRows;  // one past the last row of this launch
-    const unsigned count = static_cast<unsigned>(a.rows - a.first_row);
-    if (chunks <= 64)
-      hipLaunchKernelGGL((RowsKernel<T, kMode, 1, true>), dim3((count + 3) / 4), dim3(256), 0, stream, a);
-    else if (chunks <= 512)
-      hipLaunchKernelGGL((RowsKernel<T, kMode, 1, false>), dim3(count), threads(1), 0, stream, a);
-    else if (chunks <= 1024)
-      hipLaunchKernelGGL((RowsKernel<T, kMode, 2, false>), dim3(count), threads(2), 0, stream, a);
-    else if (chunks <= 4096)
-      hipLaunchKernelGGL((RowsKernel<T, kMode, 4, false>), dim3(count), threads(4), 0, stream, a);
-    else
-      hipLaunchKernelGGL((LongRowsKernel<T, kMode>), dim3(count), dim3(1024), 0, stream, a);
+    const unsigned count = static_cast<unsigned>(rows - a.first_row < kMostRows ? rows - a.first_row : kMostRows);
+    const dim3 blocks(count);
+    a.rows = a.first_row + count;  // one past the last row of this launch
+    if (a.width < kVec)
+      hipLaunchKernelGGL((NarrowRowsKernel<T, W, kMode, 3, true>), dim3((count + 31) / 32), dim3(256), 0, stream, a);
+    else if (chunks <= 8)
+      hipLaunchKernelGGL((NarrowRowsKernel<T, W, kMode, 3, false>), dim3((count + 31) / 32), dim3(256), 0, stream, a);
+    else if (chunks <= 16)
+      hipLaunchKernelGGL((NarrowRowsKernel<T, W, kMode, 4, false>), dim3((count + 15) / 16), dim3(256), 0, stream, a);
+    else if (chunks <= 32)
+      hipLaunchKernelGGL((NarrowRowsKernel<T, W, kMode, 5, false>), dim3((count + 7) / 8), dim3(256), 0, stream, a);
+    else if (chunks > per_thread * 1024)
+      hipLaunchKernelGGL((LongRowsKernel<T, W, kMode>), blocks, dim3(1024), 0, stream, a);
+    else if (per_thread == 1)
+      hipLaunchKernelGGL((RowsKernel<T, W, kMode, 1>), blocks, threads, 0, stream, a);
+    else if (per_thread == 2)
+      hipLaunchKernelGGL((RowsKernel<T, W, kMode, 2>), blocks, threads, 0, stream, a);
+    else if constexpr (!kWide)
+      hipLaunchKernelGGL((RowsKernel<T, W, kMode, 4>), blocks, threads, 0, stream, a);
   }
 }
 
 template <typename T>
 int LaunchMode(int mode, const RowArgs& a, hipStream_t stream) {
   switch (mode) {
-    case kPlain: LaunchRows<T, kPlain>(a, stream); break;
-    case kNorm: LaunchRows<T, kNorm>(a, stream); break;
-    case kNormResidual: LaunchRows<T, kNormResidual>(a, stream); break;
-    case kGate: LaunchRows<T, kGate>(a, stream); break;
+    case kPlain: LaunchRows<T, T, kPlain>(a, stream); break;
+    case kNorm: a.weight_f32 ? LaunchRows<T, float, kNorm>(a, stream) : LaunchRows<T, T, kNorm>(a, stream); break;
+    case kNormResidual:
+      a.weight_f32 ? LaunchRows<T, float, kNormResidual>(a, stream) : LaunchRows<T, T, kNormResidual>(a, stream);
+      break;
+    case kGate: LaunchRows<T, T, kGate>(a, stream); break;
     default: return -2;
   }
   return Status();

@@ -91,7 +91,7 @@ def _int8(rows, width, seed=0, low=-127):
     return torch.randint(low, 128, (rows, width), generator=g, dtype=torch.int8)
 
 
-WIDTHS = [1, 2, 7, 8, 9, 63, 500, 512, 513, 1000, 4095, 4096, 5000, 8192, 8200, 20001, 32768, 32769, 40000]
+WIDTHS = [1, 2, 7, 8, 9, 63, 64, 65, 120, 128, 129, 250, 256, 257, 500, 512, 513, 1000, 4095, 4096, 5000, 8192, 8200, 20001, 32768, 32769, 40000]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -102,6 +102,23 @@ def test_quantize_is_the_nearest_level(width, dtype):
     ref, top = _levels(x.float())
     assert torch.equal(q.cpu(), ref)
     assert torch.equal(scale.cpu(), top[:, 0] / 127)  # one division, correctly rounded on both sides
+
+
+@pytest.mark.parametrize("rows", [1, 31, 33, 2047, 2048, 5001])
+@pytest.mark.parametrize("width", [5, 40, 100, 200, 400, 4099])
+def test_many_rows(rows, width):
+    """The kernels that take several rows per block, and the other split of a row that many rows get."""
+    x = _values(rows, width, torch.float16, seed=rows)
+    w = _values(1, width, torch.float16, seed=1)[0]
+    q, scale = int8.quantize_int8(x.cuda())
+    ref, top = _levels(x.float())
+    assert torch.equal(q.cpu(), ref) and torch.equal(scale.cpu(), top[:, 0] / 127)
+    q, scale, h = int8.rms_norm_int8(x.cuda(), w.cuda(), residual=x.cuda())
+    want = (x.float() + x.float()).half()
+    ref, top = _levels(want.float() * w.float())
+    assert torch.equal(h.cpu(), want) and torch.equal(q.cpu(), ref)
+    factor = torch.rsqrt(want.double().square().mean(dim=-1) + 1e-6)
+    assert torch.allclose(scale.cpu().double(), top[:, 0].double() * factor / 127, rtol=1.001 * F32, atol=0)
 
 
 def test_quantize_special_rows():
@@ -147,7 +164,7 @@ def test_quantize_every_pair_of_half_values_near_borders():
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("weight_f32", [False, True])
-@pytest.mark.parametrize("width", [1, 9, 512, 1000, 4096, 5000, 8200, 32769, 40000])
+@pytest.mark.parametrize("width", [1, 9, 64, 100, 250, 512, 1000, 4096, 5000, 8200, 20001, 32769, 40000])
 def test_norm(width, dtype, weight_f32):
     x, r = _values(4, width, dtype, seed=1), _values(4, width, dtype, seed=2, spread=3.0)
     w = (1 + 0.2 * _values(1, width, torch.float32, seed=3)[0]).to(torch.float32 if weight_f32 else dtype)
@@ -203,20 +220,36 @@ def test_gate(width, dtype):
     g, u = x.double().chunk(2, dim=-1)
     p = g / (1 + torch.exp(-g)) * u
     top = p.abs().amax(dim=-1, keepdim=True)
-    # exp is good to one step (2 half steps); the sum, the quotient and the product round once each: 5 half steps on
-    # p and on the maximum, so 10 on a quotient of up to 127
-    assert ((q.double() - torch.where(top > 0, 127 * p / top, 0.0)).abs() <= 0.5 + 127 * 10.1 * F32).all()
+    # half steps: z = exp(-|g|) has 2 of the exponential unit and below 1 of its argument, 4 at most, which z / (1 + z)
+    # takes over at most once; 1 + z, g z and the quotient round once each: 7; the product with the
+    # other factor: 8 on p and on the maximum, so 16 on a quotient of up to 127 (and 9 on the scale)
+    assert ((q.double() - torch.where(top > 0, 127 * p / top, 0.0)).abs() <= 0.5 + 127 * 16.1 * F32).all()
     want = (top / 127)[:, 0]
-    assert ((scale.double() - want).abs() <= 6.1 * F32 * want + 2.0 ** -149).all()
+    assert ((scale.double() - want).abs() <= 9.1 * F32 * want + 2.0 ** -149).all()
 
 
 def test_gate_extremes():
     inf, nan = float("inf"), float("nan")
     x = torch.tensor([[-100.0, 1.0, 2.0, 3.0], [-1e4, 1.0, 2.0, 3.0], [100.0, 0.0, 2.0, 3.0], [nan, 1.0, 2.0, 3.0],
-                      [1.0, 1.0, inf, 0.0], [0.0, 0.0, 5.0, 5.0]])
+                      [1.0, 1.0, inf, 0.0], [0.0, 0.0, 5.0, 5.0], [inf, 1.0, 1.0, 1.0], [-inf, 1.0, 1.0, 1.0]])
     q, scale = (t.cpu() for t in int8.silu_mul_int8(x.cuda()))
     assert q[0].tolist() == [0, 127] and q[1].tolist() == [0, 127] and q[2].tolist() == [127, 0]
-    assert torch.isnan(scale[3:5]).all() and not q[3:].any() and scale[5] == 0
+    assert torch.isnan(scale[[3, 4, 6, 7]]).all() and not q[3:].any() and scale[5] == 0
+
+
+def test_gate_over_the_whole_range():
+    """Gates of every size, to where exp(-g) leaves fp32's range, against factors that bring the products back up."""
+    g = torch.cat([torch.linspace(-104, 89, 4001), torch.tensor([-3e38, 3e38, -1e30, 1e30, -200.5, 1e-40, -1e-40, 0.0])])
+    u = torch.full_like(g, 1e30)
+    u[g.abs() > 150] = 1e-30
+    rows = torch.stack([g, u], dim=1)  # a row each: its scale is the product's magnitude
+    scale = int8.silu_mul_int8(rows.cuda())[1].cpu().double()
+    gd = g.double()
+    # exp(-|g|) below 2^-126 is held in steps of 2^-149: half a step of it, times |g|, and half a step each for the two
+    # products behind it, at most |g| steps for the |g| > 87 at which that happens
+    want = (gd / (1 + torch.exp(-gd)) * u.double()).abs() / 127
+    coarse = torch.where(gd < 0, gd.abs() * u.double() * 2.0 ** -149 / 127, 0.0)
+    assert ((scale - want).abs() <= 9.1 * F32 * want + coarse + 2.0 ** -149).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -421,7 +454,7 @@ def test_block_together(tokens, dtype):
     g, u = y.double().chunk(2, dim=-1)
     p = g / (1 + torch.exp(-g)) * u
     t = 127 * p / p.abs().amax(dim=-1, keepdim=True)
-    assert ((q.double() - t).abs() <= 0.5 + 127 * 10.1 * F32).all()
+    assert ((q.double() - t).abs() <= 0.5 + 127 * 16.1 * F32).all()  # as in test_gate
     ref, slack = _linear_reference(q, s, w2, s2, None, h, dtype)
     assert ((out.double() - ref).abs() <= slack).all()
 
