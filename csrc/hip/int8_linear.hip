@@ -11,8 +11,8 @@
 // to lanes gives the same sum.  The weight is the MFMA's first operand: a lane then holds four consecutive outputs of
 // one token.
 //
-// SplitKernel  the waves of a block share the k axis of one small output tile: every wave multiplies its own k steps of
-//              128 straight from memory to registers, the partial sums meet in LDS.
+// SplitDmaKernel  the waves of a block share the k axis of one small output tile: every wave multiplies its own k steps of
+//              128, the sums meet in LDS.  SplitAnyKernel: the same for rows that do not start at multiples of 16 bytes.
 // TileKernel   large products: 256 x 256 (or 128 x 128) outputs per block of four waves, operands through a ring of LDS
 //              stages filled by DMA.  8192 x 8192 x 8192 to bf16: 408 us (2.69 POP/s), 462 us with a residual.  What
 //              bounds it is the card's power: on zeros, where nothing toggles, the same call takes 303 us.  One wave per
@@ -106,102 +106,37 @@ __device__ __forceinline__ void Finish(const LinearArgs& a, long long m, long lo
   else FinishFour<Bf16>(a, m, n, sum);
 }
 
-// 16 bytes of a row from k on; zeros past the row's end (bytes there may belong to nobody)
+// 16 bytes of a row from k on, zeros past the row's end.  Where the row ends among them its last 16 bytes are loaded
+// instead, and those that lie before k moved out; a row shorter than that is read one by one.
 __device__ __forceinline__ int4v LoadTail(const int8_t* row, int k, int end) {
-  int4v v = {0, 0, 0, 0};
-  if (k + 16 <= end) {
-    __builtin_memcpy(&v, row + k, 16);
+  uint64_t v[2] = {0, 0};
+  if (end >= 16) {
+    __builtin_memcpy(v, row + (k + 16 <= end ? k : end - 16), 16);
+    int past = k + 16 - end;
+    if (past > 0) {
+      if (past >= 8) {
+        v[0] = v[1];
+        v[1] = 0;
+        past -= 8;
+      }
+      if (past >= 8) v[0] = 0;
+      else if (past > 0) {
+        v[0] = v[0] >> (8 * past) | v[1] << (64 - 8 * past);
+        v[1] >>= 8 * past;
+      }
+    }
   } else {
-    unsigned char bytes[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bytes[i] = k + i < end ? static_cast<unsigned char>(row[k + i]) : 0;
-    __builtin_memcpy(&v, bytes, 16);
+    for (int i = 15; i >= 0; --i) {  // the highest first, shifted up by those below
+      v[1] = v[1] << 8 | v[0] >> 56;
+      v[0] = v[0] << 8 | (k + i < end ? static_cast<uint8_t>(row[k + i]) : 0u);
+    }
   }
-  return v;
+  int4v out;
+  __builtin_memcpy(&out, v, 16);
+  return out;
 }
 
 constexpr int kStep = 128;  // k per wave and step: a lane reads 32 consecutive bytes, four lanes a whole cache line
-
-// Block tile: 16 kMT tokens x 16 kNT outputs, k split over kWaves waves.
-template <int kMT, int kNT, int kWaves, int kAhead>
-__global__ __launch_bounds__(64 * kWaves) void SplitKernel(LinearArgs a, long long m_first, unsigned tiles_n) {
-  extern __shared__ __attribute__((aligned(16))) int4v parts[];  // [kWaves][kMT * kNT][64]
-  const unsigned tile_m = blockIdx.x / tiles_n;
-  const unsigned tile_n = blockIdx.x - tile_m * tiles_n;
-  const long long m0 = m_first + static_cast<long long>(tile_m) * (16 * kMT);
-  const long long n0 = static_cast<long long>(tile_n) * (16 * kNT);
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int8_t* xr[kMT];
-  const int8_t* wr[kNT];
-#pragma unroll
-  for (int i = 0; i < kMT; ++i) {  // rows past the end read the last one; their results are not stored
-    const long long m = m0 + i * 16 + (lane & 15);
-    xr[i] = a.x + (m < a.m ? m : a.m - 1) * a.x_stride;
-  }
-#pragma unroll
-  for (int i = 0; i < kNT; ++i) {
-    const long long n = n0 + i * 16 + (lane & 15);
-    wr[i] = a.w + (n < a.n ? n : a.n - 1) * a.w_stride;
-  }
-  int4v acc[kMT][kNT];
-#pragma unroll
-  for (int i = 0; i < kMT; ++i)
-#pragma unroll
-    for (int j = 0; j < kNT; ++j) acc[i][j] = int4v{0, 0, 0, 0};
-  const int whole = a.k / kStep;
-  const int at = (lane >> 4) * 32;
-  auto steps = [&](int s, auto count) {  // `count` steps of this wave from s on, all loads before the first product
-    constexpr int kCount = decltype(count)::value;
-    int4v x[kCount][kMT][2], w[kCount][kNT][2];
-#pragma unroll
-    for (int u = 0; u < kCount; ++u) {
-      const int k = (s + u * kWaves) * kStep + at;
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) __builtin_memcpy(w[u][j], wr[j] + k, 32);
-#pragma unroll
-      for (int i = 0; i < kMT; ++i) __builtin_memcpy(x[u][i], xr[i] + k, 32);
-    }
-#pragma unroll
-    for (int u = 0; u < kCount; ++u)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < kMT; ++i)
-#pragma unroll
-          for (int j = 0; j < kNT; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][j][h], x[u][i][h], acc[i][j], 0, 0, 0);
-  };
-  int s = wave;
-  for (; s + (kAhead - 1) * kWaves < whole; s += kAhead * kWaves) steps(s, std::integral_constant<int, kAhead>{});
-  for (; s < whole; s += kWaves) steps(s, std::integral_constant<int, 1>{});
-  if (whole * kStep < a.k && wave == whole % kWaves) {  // the last, partial step
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = whole * kStep + at + h * 16;
-      int4v x[kMT], w[kNT];
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) w[j] = LoadTail(wr[j], k, a.k);
-#pragma unroll
-      for (int i = 0; i < kMT; ++i) x[i] = LoadTail(xr[i], k, a.k);
-#pragma unroll
-      for (int i = 0; i < kMT; ++i)
-#pragma unroll
-        for (int j = 0; j < kNT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < kMT; ++i)
-#pragma unroll
-    for (int j = 0; j < kNT; ++j) parts[(wave * (kMT * kNT) + i * kNT + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  for (int f = wave; f < kMT * kNT; f += kWaves) {
-    int4v sum = parts[f * 64 + lane];
-#pragma unroll
-    for (int v = 1; v < kWaves; ++v) sum += parts[(v * (kMT * kNT) + f) * 64 + lane];
-    Finish(a, m0 + (f / kNT) * 16 + (lane & 15), n0 + (f % kNT) * 16 + (lane >> 4) * 4, sum);
-  }
-}
 
 // An offset behind every descriptor's end, also with a row's offset added: the DMA writes zeros for it, loads give zeros,
 // stores are dropped.  The host keeps the rows of a tile below 2^30 bytes.
@@ -227,10 +162,28 @@ __device__ __forceinline__ void Unrolled(F&& f) {
   }
 }
 
-// The same split over waves, operands through LDS: each wave keeps a ring of kStages steps of its own, filled by DMA.
-// The registers' way has every lane of a quarter wave in another row, so each 16 bytes are a cache lookup of their own
-// and a CU takes in 14 bytes per cycle however the loads are arranged; the DMA's lanes go along the rows, eight to a
-// 128-byte line.  No barrier until the sums meet.
+// The waves' sums of a block's tile meet in LDS, each wave's in the place of its own stages, and leave.
+template <int kMT, int kNT, int kWaves>
+__device__ __forceinline__ void MeetSums(const LinearArgs& a, long long m0, long long n0, int8_t* lds, int wave_bytes, int lane,
+                                         int wave, const int4v (&acc)[kMT][kNT]) {
+  int4v* parts = reinterpret_cast<int4v*>(lds + wave * wave_bytes);
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) parts[(i * kNT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  for (int f = wave; f < kMT * kNT; f += kWaves) {
+    int4v sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int v = 0; v < kWaves; ++v) sum += *reinterpret_cast<const int4v*>(lds + v * wave_bytes + (f * 64 + lane) * 16);
+    Finish(a, m0 + (f / kNT) * 16 + (lane & 15), n0 + (f % kNT) * 16 + (lane >> 4) * 4, sum);
+  }
+}
+
+// Block tile: 16 kMT tokens x 16 kNT outputs, k split over kWaves waves.  Each wave keeps a ring of kStages steps of its own
+// in LDS, filled by DMA, whose lanes go along the rows, eight to a 128-byte line.  (Fragments read straight from memory
+// have every lane of a quarter wave in another row: each 16 bytes are a cache lookup of their own, and a CU takes in 14
+// bytes per cycle however the loads are arranged.)  No barrier until the sums meet.
 template <int kMT, int kNT, int kWaves, int kStages>
 __global__ __launch_bounds__(64 * kWaves) void SplitDmaKernel(LinearArgs a, long long m_first, unsigned tiles_n) {
   constexpr int kXDma = 2 * kMT, kDma = 2 * (kMT + kNT);  // copies of 8 rows
@@ -301,22 +254,77 @@ __global__ __launch_bounds__(64 * kWaves) void SplitDmaKernel(LinearArgs a, long
         for (int j = 0; j < kNT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j][h], x[i][h], acc[i][j], 0, 0, 0);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  int4v* parts = reinterpret_cast<int4v*>(ring);  // own place: every arrival has been waited for
+  MeetSums<kMT, kNT, kWaves>(a, m0, n0, lds, kStages * kStageBytes, lane, wave, acc);
+}
+
+// The same for rows at any address, which the DMA does not take: a step's pieces come to registers along the rows, as the
+// DMA's lanes go, and are written to the wave's part of LDS when the step before them has been read.
+template <int kMT, int kNT, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void SplitAnyKernel(LinearArgs a, long long m_first, unsigned tiles_n) {
+  constexpr int kXPieces = 2 * kMT, kPieces = 2 * (kMT + kNT);  // 8 rows of 128 bytes each
+  constexpr int kStageBytes = kPieces * 1024;
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+  const unsigned tile_m = blockIdx.x / tiles_n;
+  const unsigned tile_n = blockIdx.x - tile_m * tiles_n;
+  const long long m0 = m_first + static_cast<long long>(tile_m) * (16 * kMT);
+  const long long n0 = static_cast<long long>(tile_n) * (16 * kNT);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int8_t* const stage = lds + wave * kStageBytes;
+  const int chunk = (lane & 7) ^ (lane >> 4);  // as in SplitDmaKernel
+  const int8_t* row[kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {  // rows past the end read the last one; their results are not stored
+    if (i < kXPieces) {
+      const long long m = m0 + i * 8 + (lane >> 3);
+      row[i] = a.x + (m < a.m ? m : a.m - 1) * a.x_stride;
+    } else {
+      const long long n = n0 + (i - kXPieces) * 8 + (lane >> 3);
+      row[i] = a.w + (n < a.n ? n : a.n - 1) * a.w_stride;
+    }
+  }
+  const int steps = (a.k + kStep - 1) / kStep;
+  int4v piece[kPieces];
+  auto load = [&](int s) {
+    if (s * kStep + kStep <= a.k) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) __builtin_memcpy(&piece[i], row[i] + s * kStep + (chunk ^ (4 * (i & 1))) * 16, 16);
+    } else if (s < steps) {  // the row ends in this step
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) piece[i] = LoadTail(row[i], s * kStep + (chunk ^ (4 * (i & 1))) * 16, a.k);
+    }
+  };
+  int4v acc[kMT][kNT];
 #pragma unroll
   for (int i = 0; i < kMT; ++i)
 #pragma unroll
-    for (int j = 0; j < kNT; ++j) parts[(i * kNT + j) * 64 + lane] = acc[i][j];
-  __syncthreads();
-  for (int f = wave; f < kMT * kNT; f += kWaves) {
-    int4v sum = {0, 0, 0, 0};
+    for (int j = 0; j < kNT; ++j) acc[i][j] = int4v{0, 0, 0, 0};
+  const int frag = (lane & 15) * kStep + ((lane >> 4) ^ ((lane >> 1) & 7)) * 16;
+  load(wave);
+  for (int s = wave; s < steps; s += kWaves) {
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) sum += *reinterpret_cast<const int4v*>(lds + v * (kStages * kStageBytes) + (f * 64 + lane) * 16);
-    Finish(a, m0 + (f / kNT) * 16 + (lane & 15), n0 + (f % kNT) * 16 + (lane >> 4) * 4, sum);
+    for (int i = 0; i < kPieces; ++i) *reinterpret_cast<int4v*>(stage + i * 1024 + lane * 16) = piece[i];
+    load(s + kWaves);
+    int4v x[kMT][2], w[kNT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int8_t* from = stage + (frag ^ (h * 64));
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) x[i][h] = *reinterpret_cast<const int4v*>(from + i * 16 * kStep);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) w[j][h] = *reinterpret_cast<const int4v*>(from + (kMT + j) * 16 * kStep);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j][h], x[i][h], acc[i][j], 0, 0, 0);
   }
+  MeetSums<kMT, kNT, kWaves>(a, m0, n0, lds, kStageBytes, lane, wave, acc);
 }
 
-// Eight consecutive values as they lie in memory.  kVector: at a multiple of 16 bytes, all inside or all outside a
-// descriptor's range; else one by one, value i at offset + i values.
+// Eight consecutive values as they lie in memory.
 template <typename T>
 struct Eight {
   static constexpr int kWords = 2 * sizeof(T);
@@ -329,50 +337,52 @@ struct Eight {
 
 using uint4v = __attribute__((ext_vector_type(4))) unsigned;
 
-// `inside` of the eight lie in the row: all or none of them with kVector
-template <typename T, bool kVector>
-__device__ __forceinline__ Eight<T> LoadEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int inside) {
+// Through a descriptor: at multiples of 16 bytes, all inside its range or (offset kOutside) not at all.
+template <typename T>
+__device__ __forceinline__ Eight<T> LoadEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset) {
   Eight<T> v;
-  auto at = [&](int i) { return static_cast<int>(i < inside ? offset + i * sizeof(T) : kOutside); };
-  if constexpr (kVector) {
 #pragma unroll
-    for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
-      const uint4v part = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(inside > 0 ? offset + 16 * i : kOutside), 0, 0);
+  for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
+    const uint4v part = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(offset + 16 * i), 0, 0);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) v.raw[4 * i + c] = part[c];
-    }
-  } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v.raw[i] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, at(i), 0, 0);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned low = static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at(2 * i), 0, 0));
-      const unsigned high = static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(rsrc, at(2 * i + 1), 0, 0));
-      v.raw[i] = low | high << 16;
-    }
+    for (int c = 0; c < 4; ++c) v.raw[4 * i + c] = part[c];
   }
   return v;
 }
 
-template <typename T, bool kVector>
-__device__ __forceinline__ void StoreEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int inside, const float (&v)[8]) {
-  T t[8];
+template <typename T>
+__device__ __forceinline__ void StoreEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, const T (&t)[8]) {
+  uint4v raw[sizeof(t) / 16];
+  __builtin_memcpy(raw, t, sizeof(t));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = FromFloat<T>(v[i]);
-  if constexpr (kVector) {
-    uint4v raw[sizeof(t) / 16];
-    __builtin_memcpy(raw, t, sizeof(t));
+  for (int i = 0; i < static_cast<int>(sizeof(t) / 16); ++i)
+    __builtin_amdgcn_raw_buffer_store_b128(raw[i], rsrc, static_cast<int>(offset + 16 * i), 0, 0);
+}
+
+// At any address, the first `inside` (at most 8, may be negative) of them.
+template <typename T>
+__device__ __forceinline__ Eight<T> LoadEight(const T* p, int inside) {
+  Eight<T> v{};
+  if (inside >= 8) {
+    __builtin_memcpy(&v, p, sizeof(v));
+  } else {
+    T t[8] = {};
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(t) / 16); ++i)
-      __builtin_amdgcn_raw_buffer_store_b128(raw[i], rsrc, static_cast<int>(inside > 0 ? offset + 16 * i : kOutside), 0, 0);
+    for (int i = 0; i < 7; ++i)
+      if (i < inside) t[i] = p[i];
+    __builtin_memcpy(&v, t, sizeof(v));
+  }
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void StoreEight(T* p, int inside, const T (&t)[8]) {
+  if (inside >= 8) {
+    __builtin_memcpy(p, t, sizeof(t));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int at = static_cast<int>(i < inside ? offset + i * sizeof(T) : kOutside);
-      if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t[i]), rsrc, at, 0, 0);
-      else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, t[i]), rsrc, at, 0, 0);
-    }
+    for (int i = 0; i < 7; ++i)
+      if (i < inside) p[i] = t[i];
   }
 }
 
@@ -429,7 +439,8 @@ __device__ __forceinline__ int Turn(int v) { return ((v ^ (v >> 1)) & 1) * 2 + (
 // Epilogue of a wave, 16 tokens at a time: the accumulators go through LDS (the wave's own part, so no barrier), after
 // which a lane holds eight consecutive outputs of a token and the lanes of a token cover whole cache lines.
 //
-// Without a residual kResidual may still be set: a descriptor of nothing gives zeros, as for a bias that is not there.
+// kVector: rows of 16-byte pieces, through descriptors, whose range ends the columns and rows of a last tile.  Without a
+// residual kResidual may still be set: zeros are added, as for a bias that is not there.
 template <typename T, bool kVector, bool kResidual, int kMT, int kNT>
 __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor& tile, int m, int n, int8_t* lds, int4v (&acc)[kMT][kNT]) {
   constexpr int kSize = sizeof(T);
@@ -443,23 +454,31 @@ __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor
   const int row = m + lane / kLanes, column = n + lane % kLanes * 8;
   const int inside = tile.columns - column;
   const auto sx_rsrc = Descriptor(a.x_scale + tile.m0, tile.rows * 4ll);
-  const auto sw_rsrc = Descriptor(a.w_scale + tile.n0, tile.columns * 4ll);
-  const auto bias_rsrc = Descriptor(a.bias ? static_cast<const T*>(a.bias) + tile.n0 : nullptr, tile.columns * kSize);
-  const auto res_rsrc = Descriptor(a.residual ? static_cast<const T*>(a.residual) + tile.m0 * a.residual_stride + tile.n0 : nullptr,
-                                   ((tile.rows - 1) * a.residual_stride + tile.columns) * kSize);
+  const T* const residual = kResidual && a.residual ? static_cast<const T*>(a.residual) + tile.m0 * a.residual_stride + tile.n0 : nullptr;
+  T* const y = static_cast<T*>(a.y) + tile.m0 * a.y_stride + tile.n0;
   // rows past the end start behind the last byte of the last one
-  const auto y_rsrc = Descriptor(static_cast<T*>(a.y) + tile.m0 * a.y_stride + tile.n0,
-                                 ((tile.rows - 1) * a.y_stride + tile.columns) * kSize);
+  const auto res_rsrc = Descriptor(residual, ((tile.rows - 1) * a.residual_stride + tile.columns) * kSize);
+  const auto y_rsrc = Descriptor(y, ((tile.rows - 1) * a.y_stride + tile.columns) * kSize);
   const unsigned y_pitch = static_cast<unsigned>(a.y_stride) * kSize, res_pitch = static_cast<unsigned>(a.residual_stride) * kSize;
-  const unsigned y_at = row * y_pitch + column * kSize, res_at = row * res_pitch + column * kSize;
+  const unsigned y_at = inside > 0 ? row * y_pitch + column * kSize : kOutside;
+  const unsigned res_at = inside > 0 ? row * res_pitch + column * kSize : kOutside;
   float sx[kMT][kTurns];
 #pragma unroll
   for (int i = 0; i < kMT; ++i)
 #pragma unroll
     for (int t = 0; t < kTurns; ++t)
       sx[i][t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sx_rsrc, (row + i * 16 + t * kRows) * 4, 0, 0));
-  const Eight<float> sw = LoadEight<float, kVector>(sw_rsrc, column * 4, inside);
-  const Eight<T> bias = LoadEight<T, kVector>(bias_rsrc, column * kSize, inside);
+  Eight<float> sw;
+  Eight<T> bias;
+  if constexpr (kVector) {
+    const auto sw_rsrc = Descriptor(a.w_scale + tile.n0, tile.columns * 4ll);
+    const auto bias_rsrc = Descriptor(a.bias ? static_cast<const T*>(a.bias) + tile.n0 : nullptr, tile.columns * kSize);
+    sw = LoadEight<float>(sw_rsrc, column * 4);
+    bias = LoadEight<T>(bias_rsrc, column * kSize);
+  } else {
+    sw = LoadEight(a.w_scale + tile.n0 + column, inside);
+    bias = LoadEight(static_cast<const T*>(a.bias) + tile.n0 + column, a.bias ? inside : 0);
+  }
   const int write = (lane & 15) * (kNT * 64);
 #pragma unroll
   for (int first = 0; first < kMT; first += kHeld) {
@@ -469,7 +488,11 @@ __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor
       for (int i = 0; i < kHeld; ++i)
 #pragma unroll
         for (int t = 0; t < kTurns; ++t)
-          if (first + i < kMT) r[i][t] = LoadEight<T, kVector>(res_rsrc, res_at + ((first + i) * 16 + t * kRows) * res_pitch, inside);
+          if (first + i < kMT) {
+            const int past = (first + i) * 16 + t * kRows;  // rows from the lane's first
+            if constexpr (kVector) r[i][t] = LoadEight<T>(res_rsrc, res_at + past * res_pitch);
+            else r[i][t] = LoadEight(residual + (row + past) * a.residual_stride + column, residual && row + past < tile.rows ? inside : 0);
+          }
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -487,13 +510,16 @@ __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum[4 * c + e] = part[e];
         }
-        float v[8];
+        T v[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          v[c] = static_cast<float>(sum[c]) * (sx[i][t] * sw[c]) + bias[c];
-          if constexpr (kResidual) v[c] += r[i - first][t][c];
+          float f = static_cast<float>(sum[c]) * (sx[i][t] * sw[c]) + bias[c];
+          if constexpr (kResidual) f += r[i - first][t][c];
+          v[c] = FromFloat<T>(f);
         }
-        StoreEight<T, kVector>(y_rsrc, y_at + (i * 16 + t * kRows) * y_pitch, inside, v);
+        const int past = i * 16 + t * kRows;
+        if constexpr (kVector) StoreEight(y_rsrc, y_at + past * y_pitch, v);
+        else StoreEight(y + (row + past) * a.y_stride + column, row + past < tile.rows ? inside : 0, v);
       }
       __builtin_amdgcn_sched_barrier(0);  // registers: no more than 16 tokens at a time
     }
@@ -674,39 +700,37 @@ int AllowLds(int bytes) {
 }
 
 // A grid holds fewer than 2^32 threads: tokens beyond that go to further launches.
-template <int kMT, int kNT, int kWaves, int kAhead>
-int LaunchSplit(const LinearArgs& a, hipStream_t stream) {
-  const long long tiles_n = (a.n + 16 * kNT - 1) / (16 * kNT);
-  constexpr long long kMostBlocks = (1ll << 31) / (64 * kWaves);
+template <int BM, int BN, int kThreads, typename F>
+int EachRun(const LinearArgs& a, F&& launch) {
+  const long long tiles_n = (a.n + BN - 1) / BN;
+  constexpr long long kMostBlocks = (1ll << 31) / kThreads;
   if (tiles_n > kMostBlocks) return -3;
-  const long long most_m = kMostBlocks / tiles_n * (16 * kMT);
-  constexpr int kLds = kWaves * kMT * kNT * 1024;
-  static_assert(kLds <= 65536, "more would have to be asked for");
+  const long long most_m = kMostBlocks / tiles_n * BM;
   for (long long m = 0; m < a.m; m += most_m) {
     const long long left = a.m - m < most_m ? a.m - m : most_m;
-    const long long blocks = (left + 16 * kMT - 1) / (16 * kMT) * tiles_n;
-    hipLaunchKernelGGL((SplitKernel<kMT, kNT, kWaves, kAhead>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves),
-                       kLds, stream, a, m, static_cast<unsigned>(tiles_n));
+    launch(static_cast<unsigned>((left + BM - 1) / BM * tiles_n), m, static_cast<unsigned>(tiles_n));
   }
   return Status();
 }
 
+template <int kMT, int kNT, int kWaves>
+int LaunchSplitAny(const LinearArgs& a, hipStream_t stream) {
+  constexpr int kLds = kWaves * (kMT + kNT) * 2048;
+  static_assert((kMT + kNT) * 2 >= kMT * kNT, "the sums meet in the stages' place");
+  if (const int rc = AllowLds<&SplitAnyKernel<kMT, kNT, kWaves>>(kLds)) return rc;
+  return EachRun<16 * kMT, 16 * kNT, 64 * kWaves>(a, [&](unsigned blocks, long long m, unsigned tiles_n) {
+    hipLaunchKernelGGL((SplitAnyKernel<kMT, kNT, kWaves>), dim3(blocks), dim3(64 * kWaves), kLds, stream, a, m, tiles_n);
+  });
+}
+
 template <int kMT, int kNT, int kWaves, int kStages>
 int LaunchSplitDma(const LinearArgs& a, hipStream_t stream) {
-  const long long tiles_n = (a.n + 16 * kNT - 1) / (16 * kNT);
-  constexpr long long kMostBlocks = (1ll << 31) / (64 * kWaves);
   constexpr int kLds = kWaves * kStages * (kMT + kNT) * 2048;
   static_assert(kLds <= 160 * 1024 && (kStages - 1) * 2 * (kMT + kNT) <= 63, "ring too large");
-  if (tiles_n > kMostBlocks) return -3;
   if (const int rc = AllowLds<&SplitDmaKernel<kMT, kNT, kWaves, kStages>>(kLds)) return rc;
-  const long long most_m = kMostBlocks / tiles_n * (16 * kMT);
-  for (long long m = 0; m < a.m; m += most_m) {
-    const long long left = a.m - m < most_m ? a.m - m : most_m;
-    const long long blocks = (left + 16 * kMT - 1) / (16 * kMT) * tiles_n;
-    hipLaunchKernelGGL((SplitDmaKernel<kMT, kNT, kWaves, kStages>), dim3(static_cast<unsigned>(blocks)), dim3(64 * kWaves), kLds,
-                       stream, a, m, static_cast<unsigned>(tiles_n));
-  }
-  return Status();
+  return EachRun<16 * kMT, 16 * kNT, 64 * kWaves>(a, [&](unsigned blocks, long long m, unsigned tiles_n) {
+    hipLaunchKernelGGL((SplitDmaKernel<kMT, kNT, kWaves, kStages>), dim3(blocks), dim3(64 * kWaves), kLds, stream, a, m, tiles_n);
+  });
 }
 
 template <typename T, int BM, int BN, int kWM, int kWN, int kStages, int kBlocks>
@@ -730,9 +754,9 @@ bool Aligned(const void* x, const void* w, long long x_stride, long long w_strid
 // Descriptors hold 32-bit offsets: 256 rows of a tile have to stay below 2^30 bytes.
 constexpr long long kMostStride = 1 << 20;
 
-// Copying the operands to aligned rows costs their bytes twice and a launch; below this the kernel that reads rows at
-// any address is as fast.
-bool Pads(long long m, long long n, long long k) { return m > 32 && m * n > (1ll << 28) / k; }
+// Copying the operands to aligned rows costs their bytes twice and a launch, and lets the tile kernel in: 26 instead of 61
+// us at 1000 x 4000 x 2001, but 12.1 both ways at 1000 x 1000 x 1001 and 18 instead of 14 at 2000 x 200 x 3001.
+bool Pads(long long m, long long n) { return m > 64 && n >= 256 && m * n > (1 << 20); }
 
 int PaddedRow(long long k) { return static_cast<int>((k + 15) / 16 * 16); }
 
@@ -746,29 +770,39 @@ int LaunchAligned(const LinearArgs& a, hipStream_t st) {
     if (fills(256, 128)) return LaunchTile<T, 256, 128, 2, 2, 4, 1>(a, st);
     if (fills(128, 128)) return LaunchTile<T, 128, 128, 2, 2, 4, 2>(a, st);
   }
-  if (a.m > 32 && fills(64, 64)) return LaunchSplitDma<4, 4, 8, 1>(a, st);
-  if (a.m > 16) {
-    if (fills(32, 64)) return LaunchSplitDma<2, 4, 8, 1>(a, st);
-    if (fills(32, 32)) return LaunchSplitDma<2, 2, 4, 2>(a, st);
-    if (fills(32, 16)) return LaunchSplitDma<2, 1, 8, 2>(a, st);
+  if (a.m > 32) {
+    if (fills(64, 128)) return LaunchTile<T, 64, 128, 2, 2, 5, 2>(a, st);
+    if (fills(64, 64)) return LaunchTile<T, 64, 64, 2, 2, 4, 4>(a, st);
   }
-  if (fills(16, 64)) return LaunchSplitDma<1, 4, 8, 1>(a, st);
-  if (fills(16, 32)) return LaunchSplitDma<1, 2, 8, 2>(a, st);
-  // waves by the length of k: each has a few steps of 128
+  // From here on k is split over the waves of a block; the more of them the longer it is, each has a few steps of 128.
+  const bool longer = a.k > 2048;
+  if (a.m > 16) {
+    if (fills(32, 64)) return longer ? LaunchSplitDma<2, 4, 8, 1>(a, st) : LaunchSplitDma<2, 4, 4, 1>(a, st);
+    if (fills(32, 32)) return longer ? LaunchSplitDma<2, 2, 4, 2>(a, st) : LaunchSplitDma<2, 2, 2, 2>(a, st);
+    if (longer && fills(32, 16)) return LaunchSplitDma<2, 1, 8, 2>(a, st);
+  } else if (fills(16, 64)) {
+    return LaunchSplitDma<1, 4, 8, 1>(a, st);
+  }
+  if (fills(16, 32)) return longer ? LaunchSplitDma<1, 2, 8, 2>(a, st) : LaunchSplitDma<1, 2, 2, 2>(a, st);
   if (a.k > 8192) return LaunchSplitDma<1, 1, 16, 2>(a, st);
-  return a.k > 1024 ? LaunchSplitDma<1, 1, 8, 2>(a, st) : LaunchSplitDma<1, 1, 4, 2>(a, st);
+  return longer ? LaunchSplitDma<1, 1, 8, 2>(a, st) : LaunchSplitDma<1, 1, 4, 2>(a, st);
 }
 
 int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
   auto fills = [&](long long bm, long long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) >= 192; };
-  if (a.m > 32 && fills(64, 64)) return LaunchSplit<4, 4, 4, 1>(a, st);
-  if (a.m > 16 && fills(32, 32)) return LaunchSplit<2, 2, 8, 1>(a, st);
-  return LaunchSplit<1, 1, 8, 2>(a, st);
+  if (a.m > 16) {
+    if (fills(32, 64)) return LaunchSplitAny<2, 4, 4>(a, st);
+    if (fills(32, 32)) return a.k > 1024 ? LaunchSplitAny<2, 2, 8>(a, st) : LaunchSplitAny<2, 2, 4>(a, st);
+  } else if (fills(16, 64)) {
+    return LaunchSplitAny<1, 4, 8>(a, st);
+  }
+  if (fills(16, 32)) return LaunchSplitAny<1, 2, 8>(a, st);
+  return a.k > 1024 ? LaunchSplitAny<1, 1, 16>(a, st) : LaunchSplitAny<1, 1, 4>(a, st);
 }
 
 int Launch(LinearArgs a, void* workspace, hipStream_t st) {
   if (!Aligned(a.x, a.w, a.x_stride, a.w_stride, a.k)) {
-    if (!Pads(a.m, a.n, a.k)) return LaunchUnaligned(a, st);
+    if (!Pads(a.m, a.n)) return LaunchUnaligned(a, st);
     if (!workspace) return -4;
     const int row = PaddedRow(a.k);
     const long long blocks = ((a.m + a.n) * (row / 16) + 255) / 256;
@@ -792,7 +826,7 @@ extern "C" {
 // Bytes of workspace (at a multiple of 16) that a launch with these operands needs; mostly 0.
 long long tca_int8_linear_workspace_bytes(const void* x, const void* w, long long m, long long n, long long k, long long x_stride,
                                           long long w_stride) {
-  if (m <= 0 || n <= 0 || k <= 0 || Aligned(x, w, x_stride, w_stride, k) || !Pads(m, n, k)) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || Aligned(x, w, x_stride, w_stride, k) || !Pads(m, n)) return 0;
   return (m + n) * PaddedRow(k);
 }
 
