@@ -99,13 +99,28 @@ __device__ __forceinline__ void Values(Chunk<T> c, int first, int width, float (
   for (int i = 0; i < kVec; ++i) v[i] = ToFloat(t[i]);
 }
 
+// N bytes to any address, by non-temporal stores: what a kernel writes does not push out what it and its neighbours are
+// still to read (norm and read-back of 16384 x 8192: 240 -> 229 us, the norm alone of 2048 x 8192 28.8 -> 22.4; a reader
+// that follows at once finds small results no later, 36.3 and 36.4 us for that norm and its read-back).
+template <int N>
+__device__ __forceinline__ void StoreBytes(void* to, const void* from) {
+  using Word = __attribute__((ext_vector_type(N >= 16 ? 4 : 2))) unsigned;
+  typedef Word AnyAddress __attribute__((aligned(1)));
+#pragma unroll
+  for (int i = 0; i < N / static_cast<int>(sizeof(Word)); ++i) {
+    Word w;
+    __builtin_memcpy(&w, static_cast<const char*>(from) + i * sizeof(Word), sizeof(Word));
+    __builtin_nontemporal_store(w, reinterpret_cast<AnyAddress*>(static_cast<char*>(to) + i * sizeof(Word)));
+  }
+}
+
 template <typename T>
 __device__ __forceinline__ void StoreChunk(T* row, int first, int width, const float (&v)[kVec]) {
   T t[kVec];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) t[i] = FromFloat<T>(v[i]);
   if (first + kVec <= width) {
-    __builtin_memcpy(row + first, t, sizeof(t));
+    StoreBytes<sizeof(t)>(row + first, t);
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
@@ -241,7 +256,7 @@ __device__ __forceinline__ uint64_t Levels(const float (&p)[kVec], float top, fl
 
 __device__ __forceinline__ void StoreLevels(int8_t* row, int first, int width, uint64_t packed) {
   if (first + kVec <= width) {
-    __builtin_memcpy(row + first, &packed, sizeof(packed));
+    StoreBytes<sizeof(packed)>(row + first, &packed);
   } else {
 #pragma unroll
     for (int i = 0; i < kVec - 1; ++i)
