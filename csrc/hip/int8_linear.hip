@@ -391,7 +391,9 @@ __device__ __forceinline__ void StoreEight(T* p, int inside, const T (&t)[8]) {
 
 // ---- TileKernel ---------------------------------------------------------------------------------------------------
 
-constexpr int kTileK = 64;  // k per stage: an LDS row of an operand is 64 bytes, one MFMA deep
+// k per stage.  An LDS row of an operand is a whole 128-byte line: the DMA takes in 105 to 130 KB per us and CU when eight
+// lanes share a line, and 60 to 70 when four do - and that is what a step's time was.
+constexpr int kTileK = 128;
 
 // The tiles of a block: each of the 8 XCDs (consecutive blocks go round them) has a contiguous run of tiles, ordered in
 // bands of kBand tile rows, so that the tiles an XCD works on at a time share operands in its L2; its blocks take them
@@ -435,9 +437,6 @@ __device__ __forceinline__ void Mfma(int4v w, int4v x, int4v& acc) {
 // touch the accumulators (16 cycles of the instruction and its write) stands here.
 __device__ __forceinline__ void SettleAccumulators() { asm volatile("s_nop 15\n\ts_nop 7"); }
 __device__ __forceinline__ void Pin(int4v& acc) { asm volatile("" : "+a"(acc)); }  // ordered with the other asm
-
-// 0, 2, 3, 1 for the low two bits 0, 1, 2, 3
-__device__ __forceinline__ int Turn(int v) { return ((v ^ (v >> 1)) & 1) * 2 + ((v >> 1) & 1); }
 
 // Epilogue of a wave, 16 tokens at a time: the accumulators go through LDS (the wave's own part, so no barrier), after
 // which a lane holds eight consecutive outputs of a token and the lanes of a token cover whole cache lines.
@@ -529,16 +528,21 @@ __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor
   }
 }
 
-// A block keeps a ring of kStages stages, each 64 k of a BM x BN tile's operands, and works through its tiles as one
+// A block keeps a ring of kStages stages, each 128 k of a BM x BN tile's operands, and works through its tiles as one
 // sequence of stages: the first stages of the next tile are on their way while this one is finished.
+//
+// A stage's two halves of 64 k are multiplied from registers.  While the second half of one is, both halves of the next are
+// read, so that its place in LDS is free for the DMA a whole stage before its products end: with two stages in LDS a request
+// has the time of one to one and a half stages to arrive.  That takes a third set of fragment registers: the first halves
+// have one, the second halves two in turn.
 template <typename T, int BM, int BN, int kWM, int kWN, int kStages, int kBlocks>
 __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs a, Tiles tiles) {
   constexpr int kWaves = kWM * kWN;
-  constexpr int kMT = BM / (16 * kWM), kNT = BN / (16 * kWN);     // fragments of a wave
-  constexpr int kXDma = BM / (16 * kWaves), kWDma = BN / (16 * kWaves);  // wave copies of 16 rows per stage
+  constexpr int kMT = BM / (16 * kWM), kNT = BN / (16 * kWN);           // fragments of a wave
+  constexpr int kXDma = BM / (8 * kWaves), kWDma = BN / (8 * kWaves);  // wave copies of 8 rows per stage
   constexpr int kDma = kXDma + kWDma;
   constexpr int kStageBytes = (BM + BN) * kTileK;
-  static_assert(kXDma >= 1 && kWDma >= 1 && (kStages - 2) * kDma <= 63, "tile does not fit the wave layout");
+  static_assert(kXDma >= 1 && kWDma >= 1 && kStages >= 2 && (kStages - 1) * kDma <= 63, "tile does not fit the wave layout");
   extern __shared__ __attribute__((aligned(16))) int8_t lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -550,19 +554,20 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
   if (tile.rows == 0) return;
   next = tile;
 
-  // Staging: copy i of a wave fills rows 16 (i kWaves + wave) .. + 15, lane l the 16 bytes at row l >> 2, place l & 3.
-  // Place of a row's 16-byte chunk: chunk ^ Turn(row >> 2).  The 16 lanes whose reads the banks serve together - four
-  // rows of each multiple of four, not all of the same chunk - then lie in 16 different 16-byte columns of the 256
-  // bytes that the banks span.
-  const int chunk = (lane & 3) ^ Turn(lane >> 4);
+  // Staging: copy i of a wave fills rows 8 (i kWaves + wave) .. + 7, lane l the 16 bytes at row l >> 3, place l & 7.  A row's
+  // chunk c lies at place c ^ ((row >> 1) & 7): the 16 lanes whose reads the banks serve together - four rows of each
+  // multiple of four, not all of the same chunk - then lie in 16 different 16-byte columns of the 256 bytes that the banks
+  // span.
+  static_assert(kWaves % 2 == 0, "a wave's rows share the parity of row >> 3");
+  const int chunk = (lane & 7) ^ (lane >> 4) ^ ((wave & 1) * 4);
   unsigned x_off[kXDma], w_off[kWDma];
 #pragma unroll
   for (int i = 0; i < kXDma; ++i)
-    x_off[i] = static_cast<unsigned>((i * kWaves + wave) * 16 + (lane >> 2)) * static_cast<unsigned>(a.x_stride);
+    x_off[i] = static_cast<unsigned>((i * kWaves + wave) * 8 + (lane >> 3)) * static_cast<unsigned>(a.x_stride);
 #pragma unroll
   for (int i = 0; i < kWDma; ++i)
-    w_off[i] = static_cast<unsigned>((i * kWaves + wave) * 16 + (lane >> 2)) * static_cast<unsigned>(a.w_stride);
-  const int span = ((a.k + kTileK - 1) / kTileK + 1) / 2 * (2 * kTileK);  // k of a tile in whole pairs of stages
+    w_off[i] = static_cast<unsigned>((i * kWaves + wave) * 8 + (lane >> 3)) * static_cast<unsigned>(a.w_stride);
+  const int stages = (a.k + kTileK - 1) / kTileK;  // of a tile
   __amdgpu_buffer_rsrc_t x_rsrc, w_rsrc;
   auto describe = [&]() {  // past the last tile: nothing, zeros arrive
     x_rsrc = Descriptor(a.x + next.m0 * a.x_stride, next.rows ? (next.rows - 1) * a.x_stride + a.k : 0);
@@ -581,7 +586,7 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
   auto issue_end = [&]() {
     issue_at = issue_at + kStageBytes == kStages * kStageBytes ? 0 : issue_at + kStageBytes;
     issue_k += kTileK;
-    if (issue_k == span) {
+    if (issue_k >= a.k) {
       issue_k = 0;
       next.at += gridDim.x >> 3;
       next.Place<BM, BN>(a, tiles);
@@ -589,43 +594,49 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
     }
   };
 
-  // Fragments: lane l holds row l & 15, k 16 (l >> 4) .. + 15
-  const int frag = (lane & 15) * kTileK + ((lane >> 4) ^ Turn(lane >> 2)) * 16;
+  // Fragments: lane l holds row l & 15, k 64 h + 16 (l >> 4) .. + 15 for half h
+  const int frag = (lane & 15) * kTileK + ((lane >> 4) ^ ((lane >> 1) & 7)) * 16;
   const int x_frag = wm * (BM / kWM) * kTileK + frag;
   const int w_frag = (BM + wn * (BN / kWN)) * kTileK + frag;
-  int4v x[2][kMT], w[2][kNT];
+  int4v x[3][kMT], w[3][kNT];
+  constexpr int kReads = kMT + kNT;  // of a half
   int read_at = 0;
-  auto read_one = [&](auto set, auto i) {
-    constexpr int s = decltype(set)::value, d = decltype(i)::value;
-    if constexpr (d < kNT) w[s][d] = *reinterpret_cast<const int4v*>(lds + read_at + w_frag + d * 16 * kTileK);
-    else x[s][d - kNT] = *reinterpret_cast<const int4v*>(lds + read_at + x_frag + (d - kNT) * 16 * kTileK);
+  auto read_one = [&](auto half, auto set, auto i) {
+    constexpr int h = decltype(half)::value, s = decltype(set)::value, d = decltype(i)::value;
+    if constexpr (d < kNT) w[s][d] = *reinterpret_cast<const int4v*>(lds + ((read_at + w_frag) ^ (h * 64)) + d * 16 * kTileK);
+    else x[s][d - kNT] = *reinterpret_cast<const int4v*>(lds + ((read_at + x_frag) ^ (h * 64)) + (d - kNT) * 16 * kTileK);
   };
   auto read_end = [&]() { read_at = read_at + kStageBytes == kStages * kStageBytes ? 0 : read_at + kStageBytes; };
 
   int4v acc[kMT][kNT];
-  // Step s: the fragments of s are in registers.  Those of s + 1 are read, stage s + kStages is requested into the
-  // place of s (read by every wave before the last barrier), both between the products.
-  auto step = [&](auto set) {
-    constexpr int cur = decltype(set)::value;
-    // A request or a read at most between two products: a product occupies its unit for 16 cycles and the wave is free to
-    // issue for 12 of them; what does not fit there leaves the unit idle.  Spread over the step: with the reads first the
-    // large product takes 472 instead of 455 us (and 322 instead of 305 on zeros).
-    constexpr int kProducts = kMT * kNT, kReads = kMT + kNT, kSlots = kReads + kDma;
+  constexpr int kProducts = kMT * kNT;  // of a half
+  // One stage; its halves are in sets 0 and `second`, the next stage's come to 0 and `third`.  A request or a read at most
+  // between two products: a product occupies its unit for 16 cycles and the wave is free to issue for 12 of them; what does
+  // not fit there leaves the unit idle.
+  auto stage = [&](auto second, auto third) {
+    constexpr int s = decltype(second)::value;
     issue_begin();
-    Unrolled<0, kProducts>([&](auto t) {
+    Unrolled<0, kProducts>([&](auto t) {  // the place of this stage has been read by every wave: requested into
       constexpr int p = decltype(t)::value, i = p / kNT, j = p % kNT;
-      Mfma(w[cur][j], x[cur][i], acc[i][j]);
-      Unrolled<p * kSlots / kProducts, (p + 1) * kSlots / kProducts>([&](auto slot) {
-        constexpr int q = decltype(slot)::value;  // the requests evenly among the reads
-        constexpr int before = (q + 1) * kDma / kSlots;
-        if constexpr (q * kDma / kSlots != before) issue_one(std::integral_constant<int, before - 1>{});
-        else read_one(std::integral_constant<int, 1 - cur>{}, std::integral_constant<int, q - before>{});
-      });
+      Mfma(w[0][j], x[0][i], acc[i][j]);
+      Unrolled<p * kDma / kProducts, (p + 1) * kDma / kProducts>(issue_one);
       __builtin_amdgcn_sched_barrier(0);
     });
     issue_end();
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kDma) : "memory");  // the next stage is there
+    __builtin_amdgcn_s_barrier();
+    Unrolled<0, kProducts>([&](auto t) {
+      constexpr int p = decltype(t)::value, i = p / kNT, j = p % kNT;
+      Mfma(w[s][j], x[s][i], acc[i][j]);
+      Unrolled<p * 2 * kReads / kProducts, (p + 1) * 2 * kReads / kProducts>([&](auto r) {
+        constexpr int q = decltype(r)::value, h = q / kReads;
+        if constexpr (h == 0) read_one(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, std::integral_constant<int, q>{});
+        else read_one(std::integral_constant<int, 1>{}, third, std::integral_constant<int, q - kReads>{});
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
     read_end();
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kDma) : "memory");
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // and has been read
     __builtin_amdgcn_s_barrier();
   };
 
@@ -637,12 +648,15 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
   }
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kDma) : "memory");
   __builtin_amdgcn_s_barrier();
-  Unrolled<0, kMT + kNT>([&](auto i) { read_one(std::integral_constant<int, 0>{}, i); });
-  read_end();
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kDma) : "memory");
-  __builtin_amdgcn_s_barrier();
 
+  constexpr std::integral_constant<int, 0> kZero{};
+  constexpr std::integral_constant<int, 1> kOne{};
+  constexpr std::integral_constant<int, 2> kTwo{};
   while (true) {
+    // The tile's first stage, here and not during the tile before: its registers serve that one's epilogue.
+    Unrolled<0, kReads>([&](auto i) { read_one(kZero, kZero, i); });
+    Unrolled<0, kReads>([&](auto i) { read_one(kOne, kOne, i); });
+    read_end();
 #pragma unroll
     for (int i = 0; i < kMT; ++i)
 #pragma unroll
@@ -651,10 +665,14 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
         Pin(acc[i][j]);
       }
     SettleAccumulators();
-    for (int k = 0; k < span; k += 2 * kTileK) {  // the last stage may be zeros
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    for (int left = stages; left > 0; left -= 2) {
+      stage(kOne, kTwo);
+      if (left == 1) break;
+      stage(kTwo, kOne);
     }
+    read_at = read_at == 0 ? (kStages - 1) * kStageBytes : read_at - kStageBytes;  // what the last stage read is read again
     SettleAccumulators();
 #pragma unroll
     for (int i = 0; i < kMT; ++i)
@@ -673,13 +691,13 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
 
 // Rows that do not start at multiples of 16 bytes are copied to rows that do, zeros behind them: the DMA moves whole
 // 16-byte pieces.  x's rows come first, w's behind them.
-__global__ __launch_bounds__(256) void PadKernel(LinearArgs a, int8_t* __restrict__ to, int pieces) {
+__global__ __launch_bounds__(256) void PadKernel(LinearArgs a, int8_t* __restrict__ to, int pieces, int pitch) {
   const long long count = (a.m + a.n) * pieces;
   for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<long long>(gridDim.x) * 256) {
     const long long row = count >> 31 ? i / pieces : static_cast<unsigned>(i) / static_cast<unsigned>(pieces);
     const int k = static_cast<int>(i - row * pieces) * 16;
     const int8_t* from = row < a.m ? a.x + row * a.x_stride : a.w + (row - a.m) * a.w_stride;
-    *reinterpret_cast<int4v*>(to + i * 16) = LoadTail(from, k, a.k);
+    *reinterpret_cast<int4v*>(to + row * pitch + k) = LoadTail(from, k, a.k);
   }
 }
 
@@ -762,7 +780,8 @@ constexpr long long kMostStride = 1 << 20;
 // us at 1000 x 4000 x 2001, but 12.1 both ways at 1000 x 1000 x 1001 and 18 instead of 14 at 2000 x 200 x 3001.
 bool Pads(long long m, long long n) { return m > 64 && n >= 256 && m * n > (1 << 20); }
 
-int PaddedRow(long long k) { return static_cast<int>((k + 15) / 16 * 16); }
+// Rows at whole lines: at other multiples of 16 every request of a line touches two (3999 x 4016 apart, 48 instead of 40 us).
+int PaddedRow(long long k) { return static_cast<int>((k + 127) / 128 * 128); }
 
 // The largest tile that leaves no more than a quarter of the 256 CUs idle, else the smallest: what a CU takes in per
 // output falls with the tile's sides, but half the CUs take in half the bytes per second.
@@ -770,13 +789,13 @@ template <typename T>
 int LaunchAligned(const LinearArgs& a, hipStream_t st) {
   auto fills = [&](long long bm, long long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) >= 192; };
   if (a.m > 64) {
-    if (fills(256, 256)) return LaunchTile<T, 256, 256, 2, 2, 4, 1>(a, st);
-    if (fills(256, 128)) return LaunchTile<T, 256, 128, 2, 2, 4, 1>(a, st);
-    if (fills(128, 128)) return LaunchTile<T, 128, 128, 2, 2, 4, 2>(a, st);
+    if (fills(256, 256)) return LaunchTile<T, 256, 256, 2, 2, 2, 1>(a, st);
+    if (fills(256, 128)) return LaunchTile<T, 256, 128, 2, 2, 3, 1>(a, st);
+    if (fills(128, 128)) return LaunchTile<T, 128, 128, 2, 2, 2, 2>(a, st);
   }
   if (a.m > 32) {
-    if (fills(64, 128)) return LaunchTile<T, 64, 128, 2, 2, 5, 2>(a, st);
-    if (fills(64, 64)) return LaunchTile<T, 64, 64, 2, 2, 4, 4>(a, st);
+    if (fills(64, 128)) return LaunchTile<T, 64, 128, 2, 2, 2, 2>(a, st);
+    if (fills(64, 64)) return LaunchTile<T, 64, 64, 2, 2, 2, 4>(a, st);
   }
   // From here on k is split over the waves of a block; the more of them the longer it is, each has a few steps of 128.
   const bool longer = a.k > 2048;
@@ -809,13 +828,14 @@ int Launch(LinearArgs a, void* workspace, hipStream_t st) {
     if (!Pads(a.m, a.n)) return LaunchUnaligned(a, st);
     if (!workspace) return -4;
     const int row = PaddedRow(a.k);
-    const long long blocks = ((a.m + a.n) * (row / 16) + 255) / 256;
+    const int pieces = (a.k + 15) / 16;
+    const long long blocks = ((a.m + a.n) * pieces + 255) / 256;
     hipLaunchKernelGGL(PadKernel, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, a,
-                       static_cast<int8_t*>(workspace), row / 16);
+                       static_cast<int8_t*>(workspace), pieces, row);
     a.x = static_cast<const int8_t*>(workspace);
     a.w = a.x + a.m * row;
     a.x_stride = a.w_stride = row;
-    a.k = row;
+    a.k = pieces * 16;
   }
   if (a.x_stride > kMostStride || a.w_stride > kMostStride || a.y_stride > kMostStride || a.residual_stride > kMostStride)
     return LaunchUnaligned(a, st);
