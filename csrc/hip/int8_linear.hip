@@ -43,6 +43,7 @@ struct LinearArgs {
   long long x_stride, w_stride, residual_stride, y_stride;
   int k;
   int dtype;
+  int pass_weight;  // few tokens: the weight is read once, and is larger than what the caches would keep of it
   int vector_rows;  // every eighth output starts at a multiple of 16 bytes, in y and the residual, and n % 8 == 0
 };
 
@@ -148,10 +149,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t Descriptor(const void* p, long
 
 using lds_ptr_t = __attribute__((address_space(3))) void*;
 
-// Wave-wide copy global -> LDS, 16 bytes per lane, to lds + 16 * lane
+// Wave-wide copy global -> LDS, 16 bytes per lane, to lds + 16 * lane; kPolicy 2: non-temporal
+template <int kPolicy = 0>
 __device__ __forceinline__ void DmaToLds(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, int8_t* lds) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, reinterpret_cast<lds_ptr_t>(reinterpret_cast<uintptr_t>(lds)), 16,
-                                           static_cast<int>(offset), 0, 0, 0);
+                                           static_cast<int>(offset), 0, 0, kPolicy);
 }
 
 template <int kFirst, int kLast, typename F>
@@ -217,6 +219,7 @@ __global__ __launch_bounds__(64 * kWaves) void SplitDmaKernel(LinearArgs a, long
     for (int i = 0; i < kDma; ++i) {
       int8_t* to = ring + stage * kStageBytes + i * 1024;
       if (i < kXDma) DmaToLds(x_rsrc, x_row + static_cast<unsigned>(i * 8 * a.x_stride) + k[i & 1], to);
+      else if (a.pass_weight) DmaToLds<2>(w_rsrc, w_row + static_cast<unsigned>((i - kXDma) * 8 * a.w_stride) + k[i & 1], to);
       else DmaToLds(w_rsrc, w_row + static_cast<unsigned>((i - kXDma) * 8 * a.w_stride) + k[i & 1], to);
     }
   };
@@ -773,6 +776,10 @@ bool Aligned(const void* x, const void* w, long long x_stride, long long w_strid
   return ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | x_stride | w_stride | k) & 15) == 0;
 }
 
+// A weight of at least half of the 256 MB behind the XCDs' caches has lost its beginning there when it is read again: 16 x
+// 32768 x 4096 takes 24.8 instead of 27.8 us past them.  One of 64 MB that is read again at once takes 14.4 instead of 12.8.
+constexpr long long kPassing = 128ll << 20;
+
 // Descriptors hold 32-bit offsets: 256 rows of a tile have to stay below 2^30 bytes.
 constexpr long long kMostStride = 1 << 20;
 
@@ -866,7 +873,8 @@ int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, co
                            ((n | y_stride | (residual ? residual_stride : 0)) & 7) == 0;
   const LinearArgs a{static_cast<const int8_t*>(x), static_cast<const float*>(x_scale), static_cast<const int8_t*>(w),
                      static_cast<const float*>(w_scale), bias, residual, y, m, n, x_stride, w_stride,
-                     residual ? residual_stride : 0, y_stride, static_cast<int>(k), dtype, vector_rows};
+                     residual ? residual_stride : 0, y_stride, static_cast<int>(k), dtype,
+                     m <= 16 && n * k >= kPassing, vector_rows};
   return Launch(a, workspace, static_cast<hipStream_t>(stream));
 }
 

@@ -294,7 +294,7 @@ LINEAR_SHAPES = [(1, 1, 1), (1, 16, 64), (1, 4096, 4096), (2, 3, 15), (3, 17, 16
                  (15, 100, 127), (16, 64, 128), (17, 65, 129), (32, 128, 255), (33, 130, 256), (48, 500, 1001),
                  (63, 63, 63), (64, 64, 640), (65, 1000, 513), (100, 257, 2000), (128, 128, 128), (129, 384, 1024),
                  (200, 1000, 2049), (256, 256, 96), (257, 513, 4000), (300, 1000, 2048), (500, 2048, 1040),
-                 (777, 777, 777), (1024, 1024, 512), (1025, 2050, 1056)]
+                 (777, 777, 777), (1024, 1024, 512), (1025, 2050, 1056), (5, 33000, 4096)]
 
 
 @pytest.mark.parametrize("m,n,k", LINEAR_SHAPES)
