@@ -63,6 +63,21 @@ void* CurrentStream(int device) { return c10::hip::getCurrentHIPStream(static_ca
 
 #define NOT_PLAIN Py_RETURN_NONE
 
+// a tuple of the results, or null where one could not be made
+template <typename... Results>
+PyObject* Tuple(Results&&... results) {
+  const py::object made[] = {py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(results)))...};
+  PyObject* tuple = PyTuple_New(sizeof...(results));
+  for (Py_ssize_t i = 0; tuple && i < static_cast<Py_ssize_t>(sizeof...(results)); ++i) {
+    if (!made[i]) {
+      Py_CLEAR(tuple);
+      break;
+    }
+    PyTuple_SET_ITEM(tuple, i, py::object(made[i]).release().ptr());
+  }
+  return tuple;
+}
+
 // (x, gated) -> (q, scale)
 PyObject* Quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -83,8 +98,7 @@ PyObject* Quantize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (rows && g_quantize(x->const_data_ptr(), q.mutable_data_ptr(), scale.mutable_data_ptr(), code, gated, rows, width,
                          sizes.back(), width, CurrentStream(device)))
     NOT_PLAIN;
-  return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(q))).ptr(),
-                      py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(scale))).ptr());
+  return Tuple(q, scale);
   END_HANDLE_TH_ERRORS
 }
 
@@ -117,11 +131,7 @@ PyObject* Norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
                      weight->scalar_type() == at::kFloat, eps, rows, width, width, with_residual ? width : 0, width,
                      with_residual ? width : 0, CurrentStream(device)))
     NOT_PLAIN;
-  const auto wrapped_q = py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(q)));
-  const auto wrapped_scale = py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(scale)));
-  if (!with_residual) return PyTuple_Pack(2, wrapped_q.ptr(), wrapped_scale.ptr());
-  return PyTuple_Pack(3, wrapped_q.ptr(), wrapped_scale.ptr(),
-                      py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(sum))).ptr());
+  return with_residual ? Tuple(q, scale, sum) : Tuple(q, scale);
   END_HANDLE_TH_ERRORS
 }
 

@@ -535,3 +535,183 @@ def test_offsets_beyond_32_bits():
     b, sb = _int8(60000, 16, seed=2).cuda(), torch.rand(60000).cuda()
     y = int8.linear_int8(a, sa, b, sb)
     assert torch.equal(y[-300:], int8.linear_int8(a[-300:].clone(), sa[-300:], b, sb))
+
+
+# outputs that take each of the tiles of a large product: 256 x 256, 256 x 128, 128 x 128, 64 x 128, 64 x 64
+TILED = [(3600, 3592), (2500, 2600), (1500, 2000), (1000, 1600), (500, 2000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("k", [16, 128, 272, 400])  # one stage of 128 and less, odd and even numbers of them
+@pytest.mark.parametrize("m,n", TILED)
+def test_linear_in_each_tile(m, n, k, dtype):
+    for cut in (0, 4, 1):  # outputs of a row: a multiple of 8, of 4, odd
+        _linear_case(m - cut, n - cut, k, dtype, bias=cut != 4, residual=True, seed=cut)
+    _linear_case(m, n, k - 1, dtype, bias=True, seed=k)  # copied to aligned rows
+    _linear_case(m, n, k, dtype)
+
+
+@pytest.mark.parametrize("m,n", [(9, 40), (70, 300), (520, 2000), (2500, 2600)])
+def test_linear_with_rows_of_one_place(m, n):
+    """Broadcast operands: every row of x, of the residual, or of the weight is the same one."""
+    k = 144
+    x, w = _int8(1, k, seed=1).cuda().expand(m, k), _int8(n, k, seed=2).cuda()
+    xs, ws = torch.rand(m).cuda() * 0.01, (torch.rand(1).cuda() * 0.01).expand(n)
+    r = torch.randn(1, n, device="cuda").bfloat16().expand(m, n)
+    y = int8.linear_int8(x, xs, w, ws, residual=r, dtype=torch.bfloat16)
+    ref, slack = _linear_reference(x, xs, w, ws, None, r, torch.bfloat16)
+    assert ((y.double() - ref).abs() <= slack).all()
+    one = _int8(1, k, seed=3).cuda()
+    y = int8.linear_int8(x.contiguous(), xs, one.expand(n, k), ws, bias=r[0], dtype=torch.bfloat16)
+    ref, slack = _linear_reference(x, xs, one.expand(n, k), ws, r[0], None, torch.bfloat16)
+    assert ((y.double() - ref).abs() <= slack).all()
+
+
+@pytest.mark.parametrize("far", ["x", "weight", "residual", "out"])
+def test_linear_rows_far_apart(far):
+    """Rows more than 2^20 apart, where a tile's offsets would leave the range of its descriptors."""
+    m, n, k, stride = 300, 280, 160, (1 << 20) + 32
+    x, w = _int8(m, k, seed=1).cuda(), _int8(n, k, seed=2).cuda()
+    xs, ws = torch.rand(m).cuda() * 0.01, torch.rand(n).cuda() * 0.01
+    r = torch.randn(m, n, device="cuda").half()
+
+    def apart(t):
+        to = torch.zeros((t.shape[0] - 1) * stride + t.shape[1], dtype=t.dtype, device="cuda").as_strided(t.shape, (stride, 1))
+        to.copy_(t)
+        return to
+
+    want = int8.linear_int8(x, xs, w, ws, residual=r)
+    out = None
+    if far == "x":
+        x = apart(x)
+    elif far == "weight":
+        w = apart(w)
+    elif far == "residual":
+        r = apart(r)
+    else:
+        out = apart(torch.empty_like(r))
+    assert torch.equal(int8.linear_int8(x, xs, w, ws, residual=r, out=out), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("width", [4096, 8190, 16384, 20000])
+def test_many_wide_rows(width, dtype):
+    """2048 rows and more: several chunks of a row per thread, in every operator and type."""
+    rows = 2050
+    x, r = _values(rows, width, dtype, seed=1), _values(rows, width, dtype, seed=2)
+    w = (1 + 0.2 * _values(1, width, torch.float32, seed=3)[0]).to(dtype)
+    xd, rd, wd = x.cuda(), r.cuda(), w.cuda()
+    few = [int8.quantize_int8(xd[:7]), int8.rms_norm_int8(xd[:7], wd), int8.rms_norm_int8(xd[:7], wd.float(), residual=rd[:7])]
+    many = [int8.quantize_int8(xd), int8.rms_norm_int8(xd, wd), int8.rms_norm_int8(xd, wd.float(), residual=rd)]
+    for a, b in zip(few, many):  # one well-defined answer, but for the order of the squares' sum in 64 bits
+        assert torch.equal(a[0], b[0][:7])
+        assert ((a[1].double() - b[1][:7].double()).abs() <= 2.002 * F32 * a[1].double()).all()
+    assert torch.equal(few[2][2], many[2][2][:7])
+    last = slice(rows - 5, rows)
+    for (q, scale, *h), p, norm_of in ((many[0], x[last].float(), None), (many[1], x[last].float() * w.float(), x[last]),
+                                       (many[2], (x[last].float() + r[last].float()).to(dtype).float() * w.float(),
+                                        (x[last].float() + r[last].float()).to(dtype))):
+        ref, top = _levels(p)
+        assert torch.equal(q[last].cpu(), ref)
+        want = top[:, 0].double() / 127
+        if norm_of is not None:
+            want = want * torch.rsqrt(norm_of.double().square().mean(dim=-1) + 1e-6)
+        assert ((scale[last].cpu().double() - want).abs() <= 1.001 * F32 * want).all()
+    q, scale = int8.silu_mul_int8(xd)
+    few_q, few_scale = int8.silu_mul_int8(xd[-7:])
+    if width % 2 == 0:
+        assert torch.equal(q[-7:], few_q) and torch.equal(scale[-7:], few_scale)
+
+
+def test_two_threads_at_once():
+    """Calls of two threads, each on a stream of its own, with workspaces in flight."""
+    import threading
+
+    cases = []
+    for s in range(2):
+        x, w = _int8(1100, 333, seed=s).cuda(), _int8(1201, 333, seed=5 + s).cuda()
+        xs, ws = torch.rand(1100).cuda(), torch.rand(1201).cuda()
+        cases.append((x, xs, w, ws, int8.linear_int8(x, xs, w, ws, dtype=torch.bfloat16)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(x, xs, w, ws, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    y = int8.linear_int8(x, xs, w, ws, dtype=torch.bfloat16)
+                    q, s = int8.quantize_int8(y)
+                    back = int8.dequantize_int8(q, s, dtype=torch.float32)
+                    if not torch.equal(y, want) or ((back - want.float()).abs() > 0.51 * s[:, None]).any():
+                        bad.append("a result differs")
+        except Exception as e:  # noqa: BLE001 - reported by the test's own thread
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_copied_rows_in_a_graph():
+    """A product whose operands are copied to a workspace, captured twice, replayed with eager ones between."""
+    m, n, k = 1100, 1200, 333
+    w, ws = _int8(n, k, seed=1).cuda(), torch.rand(n).cuda()
+    xs = torch.rand(m).cuda()
+    inputs = [_int8(m, k, seed=10 + i).cuda() for i in range(3)]
+    want = [int8.linear_int8(x, xs, w, ws) for x in inputs]
+    graphs = []
+    for _ in range(2):
+        x_in = inputs[0].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = int8.linear_int8(x_in, xs, w, ws)
+        graphs.append((graph, x_in, y))
+    for turn in range(6):
+        for i, (graph, x_in, y) in enumerate(graphs):
+            at = (turn + i) % 3
+            x_in.copy_(inputs[at])
+            graph.replay()
+            assert torch.equal(int8.linear_int8(inputs[at], xs, w, ws), want[at])
+            assert torch.equal(y, want[at])
+
+
+def test_first_call_inside_a_capture():
+    """In a process of its own: a kernel's LDS is allowed, and the extension loaded, while a stream is captured."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from triton_client_amd.ops import int8
+x = torch.randint(-127, 128, (2000, 256), dtype=torch.int8, device="cuda")
+s = torch.full((2000,), 0.01, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = int8.linear_int8(x, s, x, s, dtype=torch.float32)
+    q, t = int8.quantize_int8(y)
+for _ in range(3):
+    y.fill_(0)
+    graph.replay()
+    torch.cuda.synchronize()
+    eager = int8.linear_int8(x, s, x, s, dtype=torch.float32)
+    assert torch.equal(y, eager) and torch.equal(q, int8.quantize_int8(eager)[0])
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]
+
+
+def test_parameters_without_gradients():
+    """Parameters are operands like any other where no gradient is recorded, and results require none."""
+    x = torch.nn.Parameter(_values(6, 64, torch.float16).cuda())
+    w = torch.nn.Parameter(torch.ones(64, dtype=torch.float16, device="cuda"))
+    with torch.no_grad():
+        got = int8.rms_norm_int8(x, w, residual=x)
+    for a, b in zip(got, int8.rms_norm_int8(x.detach(), w.detach(), residual=x.detach())):
+        assert torch.equal(a, b) and not a.requires_grad
+    frozen = torch.nn.Parameter(x.detach(), requires_grad=False)
+    assert torch.equal(int8.quantize_int8(frozen)[0], int8.quantize_int8(x.detach())[0])

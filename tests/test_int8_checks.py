@@ -121,3 +121,15 @@ def test_destinations_lie_apart():
         int8._check_apart((("out", base[1:], (base,)),), (base,))
     with pytest.raises(ValueError, match="scale overlaps out"):
         int8._check_apart((("out", base, ()), ("scale", base[0], ())), ())
+
+
+def test_pending_negations_are_refused():
+    """A view whose negation is pending shows other values than those in memory."""
+    x = torch._neg_view(torch.ones(2, 8))
+    for call in (lambda: int8.quantize_int8(x), lambda: int8.silu_mul_int8(x),
+                 lambda: int8.rms_norm_int8(torch.ones(2, 8), x[0]),
+                 lambda: int8.dequantize_int8(_x(2, 8, dtype=torch.int8), x[:, 0]),
+                 lambda: _linear(dtype=torch.float32, bias=x[0, :4]),
+                 lambda: _linear(x_scale=x[0, :3]), lambda: _linear(weight_scale=x[0, :4])):
+        with pytest.raises(ValueError, match="negation"):
+            call()

@@ -59,14 +59,15 @@ def _output_code(dtype):
 
 
 def _check_operands(first, others):
-    """Index of the operands' common CUDA device; no operand may require a gradient while gradients are recorded."""
+    """Index of the operands' common CUDA device; no operand may require a gradient while gradients are recorded, nor
+    stand for other values than those in memory."""
     device = first.get_device()
-    if first.requires_grad:
-        _refuse_gradient()
-    for t in others:
+    for t in (first, *others):
         if t is not None:
             if t.requires_grad:
                 _refuse_gradient()
+            if t.is_neg():
+                raise ValueError("an operand's negation is pending: call its resolve_neg()")
             if t.get_device() != device:
                 raise ValueError("the operands must be on one device")
     if device < 0:
