@@ -44,7 +44,8 @@ struct LinearArgs {
   int k;
   int dtype;
   int pass_weight;  // few tokens: the weight is read once, and is larger than what the caches would keep of it
-  int vector_rows;  // every eighth output starts at a multiple of 16 bytes, in y and the residual, and n % 8 == 0
+  int vector_rows;  // 16 bytes of outputs start at a multiple of 16 bytes, in y and the residual, and end with the row
+  int line_rows;    // every row of y starts at a whole line
 };
 
 struct Bf16 {
@@ -107,30 +108,38 @@ __device__ __forceinline__ void Finish(const LinearArgs& a, long long m, long lo
   else FinishFour<Bf16>(a, m, n, sum);
 }
 
-// 16 bytes of a row from k on, zeros past the row's end.  Where the row ends among them its last 16 bytes are loaded
-// instead, and those that lie before k moved out; a row shorter than that is read one by one.
-__device__ __forceinline__ int4v LoadTail(const int8_t* row, int k, int end) {
+// 16 bytes of a row from k on, in two steps, so that several requests can be on their way.  Where the row ends among them
+// its last 16 bytes are requested instead; a row shorter than that is read one by one.
+__device__ __forceinline__ int4v RequestPiece(const int8_t* row, int k, int end) {
   uint64_t v[2] = {0, 0};
   if (end >= 16) {
     __builtin_memcpy(v, row + (k + 16 <= end ? k : end - 16), 16);
-    int past = k + 16 - end;
-    if (past > 0) {
-      if (past >= 8) {
-        v[0] = v[1];
-        v[1] = 0;
-        past -= 8;
-      }
-      if (past >= 8) v[0] = 0;
-      else if (past > 0) {
-        v[0] = v[0] >> (8 * past) | v[1] << (64 - 8 * past);
-        v[1] >>= 8 * past;
-      }
-    }
   } else {
     for (int i = 15; i >= 0; --i) {  // the highest first, shifted up by those below
       v[1] = v[1] << 8 | v[0] >> 56;
       v[0] = v[0] << 8 | (k + i < end ? static_cast<uint8_t>(row[k + i]) : 0u);
     }
+  }
+  int4v out;
+  __builtin_memcpy(&out, v, 16);
+  return out;
+}
+
+// What was requested, those that lie before k moved out and zeros past the row's end.
+__device__ __forceinline__ int4v PieceOf(int4v requested, int k, int end) {
+  int past = k + 16 - end;
+  if (end < 16 || past <= 0) return requested;
+  uint64_t v[2];
+  __builtin_memcpy(v, &requested, 16);
+  if (past >= 8) {
+    v[0] = v[1];
+    v[1] = 0;
+    past -= 8;
+  }
+  if (past >= 8) v[0] = 0;
+  else if (past > 0) {
+    v[0] = v[0] >> (8 * past) | v[1] << (64 - 8 * past);
+    v[1] >>= 8 * past;
   }
   int4v out;
   __builtin_memcpy(&out, v, 16);
@@ -294,7 +303,10 @@ __global__ __launch_bounds__(64 * kWaves) void SplitAnyKernel(LinearArgs a, long
       for (int i = 0; i < kPieces; ++i) __builtin_memcpy(&piece[i], row[i] + s * kStep + (chunk ^ (4 * (i & 1))) * 16, 16);
     } else if (s < steps) {  // the row ends in this step
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) piece[i] = LoadTail(row[i], s * kStep + (chunk ^ (4 * (i & 1))) * 16, a.k);
+      for (int i = 0; i < kPieces; ++i) {
+        const int k = s * kStep + (chunk ^ (4 * (i & 1))) * 16;
+        piece[i] = PieceOf(RequestPiece(row[i], k, a.k), k, a.k);
+      }
     }
   };
   int4v acc[kMT][kNT];
@@ -327,11 +339,11 @@ __global__ __launch_bounds__(64 * kWaves) void SplitAnyKernel(LinearArgs a, long
   MeetSums<kMT, kNT, kWaves>(a, m0, n0, lds, kStageBytes, lane, wave, acc);
 }
 
-// Eight consecutive values as they lie in memory.
+// 16 bytes of consecutive values as they lie in memory.
 template <typename T>
-struct Eight {
-  static constexpr int kWords = 2 * sizeof(T);
-  unsigned raw[kWords];
+struct Part {
+  static constexpr int kValues = 16 / sizeof(T);
+  unsigned raw[4] = {};
   __device__ __forceinline__ float operator[](int i) const {
     if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i]);
     else return ToFloat(__builtin_bit_cast(T, static_cast<unsigned short>(raw[i / 2] >> (16 * (i & 1)))));
@@ -342,54 +354,28 @@ using uint4v = __attribute__((ext_vector_type(4))) unsigned;
 
 // Through a descriptor: at multiples of 16 bytes, all inside its range or (offset kOutside) not at all.
 template <typename T>
-__device__ __forceinline__ Eight<T> LoadEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset) {
-  Eight<T> v;
+__device__ __forceinline__ Part<T> LoadPart(__amdgpu_buffer_rsrc_t rsrc, unsigned offset) {
+  const uint4v raw = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(offset), 0, 0);
+  Part<T> v;
 #pragma unroll
-  for (int i = 0; i < Eight<T>::kWords / 4; ++i) {
-    const uint4v part = __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(offset + 16 * i), 0, 0);
-#pragma unroll
-    for (int c = 0; c < 4; ++c) v.raw[4 * i + c] = part[c];
-  }
+  for (int c = 0; c < 4; ++c) v.raw[c] = raw[c];
   return v;
 }
 
-// Non-temporal: what is written leaves the operands and residuals of the neighbours their places in the caches (8192 x 8192
-// x 8192 with a residual 466 -> 427 us, 4096 x 4096 x 4096 61.3 -> 59.4).
+// At any address, the first `inside` (may be more, or negative) of them.
 template <typename T>
-__device__ __forceinline__ void StoreEight(__amdgpu_buffer_rsrc_t rsrc, unsigned offset, const T (&t)[8]) {
-  constexpr int kNonTemporal = 2;
-  uint4v raw[sizeof(t) / 16];
-  __builtin_memcpy(raw, t, sizeof(t));
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(t) / 16); ++i)
-    __builtin_amdgcn_raw_buffer_store_b128(raw[i], rsrc, static_cast<int>(offset + 16 * i), 0, kNonTemporal);
-}
-
-// At any address, the first `inside` (at most 8, may be negative) of them.
-template <typename T>
-__device__ __forceinline__ Eight<T> LoadEight(const T* p, int inside) {
-  Eight<T> v{};
-  if (inside >= 8) {
-    __builtin_memcpy(&v, p, sizeof(v));
+__device__ __forceinline__ Part<T> LoadPart(const T* p, int inside) {
+  Part<T> v;
+  if (inside >= Part<T>::kValues) {
+    __builtin_memcpy(v.raw, p, 16);
   } else {
-    T t[8] = {};
+    T t[Part<T>::kValues] = {};
 #pragma unroll
-    for (int i = 0; i < 7; ++i)
+    for (int i = 0; i < Part<T>::kValues - 1; ++i)
       if (i < inside) t[i] = p[i];
-    __builtin_memcpy(&v, t, sizeof(v));
+    __builtin_memcpy(v.raw, t, 16);
   }
   return v;
-}
-
-template <typename T>
-__device__ __forceinline__ void StoreEight(T* p, int inside, const T (&t)[8]) {
-  if (inside >= 8) {
-    __builtin_memcpy(p, t, sizeof(t));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (i < inside) p[i] = t[i];
-  }
 }
 
 // ---- TileKernel ---------------------------------------------------------------------------------------------------
@@ -441,63 +427,95 @@ __device__ __forceinline__ void Mfma(int4v w, int4v x, int4v& acc) {
 __device__ __forceinline__ void SettleAccumulators() { asm volatile("s_nop 15\n\ts_nop 7"); }
 __device__ __forceinline__ void Pin(int4v& acc) { asm volatile("" : "+a"(acc)); }  // ordered with the other asm
 
+// How the rows of outputs and residuals lie: at whole 128-byte lines, at multiples of 16 bytes, at any address.
+enum Rows : int { kLines, kPieces, kAny };
+
 // Epilogue of a wave, 16 tokens at a time: the accumulators go through LDS (the wave's own part, so no barrier), after
-// which a lane holds eight consecutive outputs of a token and the lanes of a token cover whole cache lines.
+// which a lane holds 16 bytes of consecutive outputs of a token (fp32: two such parts, half of the wave's columns apart)
+// and the lanes of a token cover whole cache lines.
 //
-// kVector: rows of 16-byte pieces, through descriptors, whose range ends the columns and rows of a last tile.  Without a
-// residual kResidual may still be set: zeros are added, as for a bias that is not there.
-template <typename T, bool kVector, bool kResidual, int kMT, int kNT>
+// kLines, kPieces: through descriptors, whose range ends the columns and rows of a last tile.  Results that fill whole lines
+// are stored past the caches and leave the neighbours' operands and residuals their places there (8192 x 8192 x 8192 with a
+// residual 466 -> 427 us); parts of lines cost twice the time that way.  Without a residual kResidual may still be set:
+// zeros are added, as for a bias that is not there.
+template <typename T, int kRowsAt, bool kResidual, int kMT, int kNT>
 __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor& tile, int m, int n, int8_t* lds, int4v (&acc)[kMT][kNT]) {
   constexpr int kSize = sizeof(T);
+  constexpr int kPer = Part<T>::kValues, kParts = 8 / kPer;  // a lane's eight outputs
   constexpr int kLanes = kNT * 2;               // lanes of a token
   constexpr int kRows = 64 / kLanes;            // tokens of one access
   constexpr int kTurns = 16 / kRows;            // accesses for 16 tokens
   constexpr int kTurnMask = kNT * 4 < 16 ? kNT * 4 - 1 : 15;
-  constexpr int kHeld = !kVector ? 1 : kSize == 2 ? 4 : 2;  // steps of 16 tokens whose residual is requested at once
+  constexpr int kHeld = kSize == 2 ? 4 : 2;     // steps of 16 tokens whose residual is requested at once
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));  // addresses are computed here for every tile: kept from tile to tile they would spill
-  const int row = m + lane / kLanes, column = n + lane % kLanes * 8;
-  const int inside = tile.columns - column;
+  const int row = m + lane / kLanes;
   const auto sx_rsrc = Descriptor(a.x_scale + tile.m0, tile.rows * 4ll);
   const T* const residual = kResidual && a.residual ? static_cast<const T*>(a.residual) + tile.m0 * a.residual_stride + tile.n0 : nullptr;
   T* const y = static_cast<T*>(a.y) + tile.m0 * a.y_stride + tile.n0;
+  const T* const bias_row = a.bias ? static_cast<const T*>(a.bias) + tile.n0 : nullptr;
   // rows past the end start behind the last byte of the last one
   const auto res_rsrc = Descriptor(residual, ((tile.rows - 1) * a.residual_stride + tile.columns) * kSize);
   const auto y_rsrc = Descriptor(y, ((tile.rows - 1) * a.y_stride + tile.columns) * kSize);
   const unsigned y_pitch = static_cast<unsigned>(a.y_stride) * kSize, res_pitch = static_cast<unsigned>(a.residual_stride) * kSize;
-  const unsigned y_at = inside > 0 ? row * y_pitch + column * kSize : kOutside;
-  const unsigned res_at = inside > 0 ? row * res_pitch + column * kSize : kOutside;
+  int column[kParts], inside[kParts];
+  unsigned y_at[kParts], res_at[kParts];
+  float sw[8];
+  Part<T> bias[kParts];
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) {
+    column[p] = n + (p * kLanes + lane % kLanes) * kPer;
+    inside[p] = tile.columns - column[p];
+    if constexpr (kRowsAt != kAny) {
+      y_at[p] = inside[p] > 0 ? row * y_pitch + column[p] * kSize : kOutside;
+      res_at[p] = inside[p] > 0 ? row * res_pitch + column[p] * kSize : kOutside;
+      const auto sw_rsrc = Descriptor(a.w_scale + tile.n0, tile.columns * 4ll);
+      bias[p] = LoadPart<T>(Descriptor(bias_row, tile.columns * kSize), column[p] * kSize);
+#pragma unroll
+      for (int c = 0; c < kPer; c += 4) {
+        const Part<float> four = LoadPart<float>(sw_rsrc, (column[p] + c) * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sw[p * kPer + c + e] = four[e];
+      }
+    } else {
+      bias[p] = LoadPart(bias_row + column[p], bias_row ? inside[p] : 0);
+#pragma unroll
+      for (int c = 0; c < kPer; c += 4) {
+        const Part<float> four = LoadPart(a.w_scale + tile.n0 + column[p] + c, inside[p] - c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sw[p * kPer + c + e] = four[e];
+      }
+    }
+  }
+  const bool ragged = kRowsAt == kAny && tile.columns % kPer != 0;  // some lane's part ends inside its 16 bytes
   float sx[kMT][kTurns];
 #pragma unroll
   for (int i = 0; i < kMT; ++i)
 #pragma unroll
     for (int t = 0; t < kTurns; ++t)
       sx[i][t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sx_rsrc, (row + i * 16 + t * kRows) * 4, 0, 0));
-  Eight<float> sw;
-  Eight<T> bias;
-  if constexpr (kVector) {
-    const auto sw_rsrc = Descriptor(a.w_scale + tile.n0, tile.columns * 4ll);
-    const auto bias_rsrc = Descriptor(a.bias ? static_cast<const T*>(a.bias) + tile.n0 : nullptr, tile.columns * kSize);
-    sw = LoadEight<float>(sw_rsrc, column * 4);
-    bias = LoadEight<T>(bias_rsrc, column * kSize);
-  } else {
-    sw = LoadEight(a.w_scale + tile.n0 + column, inside);
-    bias = LoadEight(static_cast<const T*>(a.bias) + tile.n0 + column, a.bias ? inside : 0);
-  }
   const int write = (lane & 15) * (kNT * 64);
 #pragma unroll
   for (int first = 0; first < kMT; first += kHeld) {
-    Eight<T> r[kHeld][kTurns];
+    Part<T> r[kHeld][kTurns][kParts];
     if constexpr (kResidual) {
 #pragma unroll
       for (int i = 0; i < kHeld; ++i)
 #pragma unroll
         for (int t = 0; t < kTurns; ++t)
-          if (first + i < kMT) {
-            const int past = (first + i) * 16 + t * kRows;  // rows from the lane's first
-            if constexpr (kVector) r[i][t] = LoadEight<T>(res_rsrc, res_at + past * res_pitch);
-            else r[i][t] = LoadEight(residual + (row + past) * a.residual_stride + column, residual && row + past < tile.rows ? inside : 0);
-          }
+#pragma unroll
+          for (int p = 0; p < kParts; ++p)
+            if (first + i < kMT) {
+              const int past = (first + i) * 16 + t * kRows;  // rows from the lane's first
+              if constexpr (kRowsAt != kAny) {
+                r[i][t][p] = LoadPart<T>(res_rsrc, res_at[p] + past * res_pitch);
+              } else if (residual) {
+                // rows and parts past the end read others, whose sums are not stored; no branch, so all are on their way
+                const char* from = reinterpret_cast<const char*>(residual) + min(row + past, tile.rows - 1) * res_pitch;
+                if (tile.columns >= kPer) __builtin_memcpy(r[i][t][p].raw, from + (inside[p] >= kPer ? column[p] * kSize : 0), 16);
+                if (ragged && inside[p] < kPer) r[i][t][p] = LoadPart(reinterpret_cast<const T*>(from) + column[p], inside[p]);
+              }
+            }
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
@@ -508,23 +526,37 @@ __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor
 #pragma unroll
       for (int t = 0; t < kTurns; ++t) {
         const int from = lane / kLanes + t * kRows;
-        int sum[8];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int4v part = *reinterpret_cast<const int4v*>(lds + from * (kNT * 64) + ((lane % kLanes * 2 + c) ^ (from & kTurnMask)) * 16);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[4 * c + e] = part[e];
-        }
-        T v[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          float f = static_cast<float>(sum[c]) * (sx[i][t] * sw[c]) + bias[c];
-          if constexpr (kResidual) f += r[i - first][t][c];
-          v[c] = FromFloat<T>(f);
-        }
         const int past = i * 16 + t * kRows;
-        if constexpr (kVector) StoreEight(y_rsrc, y_at + past * y_pitch, v);
-        else StoreEight(y + (row + past) * a.y_stride + column, row + past < tile.rows ? inside : 0, v);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+          T v[kPer];
+#pragma unroll
+          for (int c = 0; c < kPer; c += 4) {
+            const int at = kParts == 1 ? lane % kLanes * 2 + c / 4 : p * kLanes + lane % kLanes;
+            const int4v sum = *reinterpret_cast<const int4v*>(lds + from * (kNT * 64) + (at ^ (from & kTurnMask)) * 16);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float f = static_cast<float>(sum[e]) * (sx[i][t] * sw[p * kPer + c + e]) + bias[p][c + e];
+              if constexpr (kResidual) f += r[i - first][t][p][c + e];
+              v[c + e] = FromFloat<T>(f);
+            }
+          }
+          if constexpr (kRowsAt != kAny) {
+            uint4v raw;
+            __builtin_memcpy(&raw, v, 16);
+            __builtin_amdgcn_raw_buffer_store_b128(raw, y_rsrc, static_cast<int>(y_at[p] + past * y_pitch), 0,
+                                                   kRowsAt == kLines ? 2 : 0);  // 2: non-temporal
+          } else if (row + past < tile.rows) {
+            T* const to = reinterpret_cast<T*>(reinterpret_cast<char*>(y) + static_cast<unsigned>(row + past) * y_pitch) + column[p];
+            if (inside[p] >= kPer) __builtin_memcpy(to, v, 16);
+            asm volatile("");  // or the two kinds of stores are merged, into many small ones
+            if (ragged && inside[p] < kPer) {
+#pragma unroll
+              for (int c = 0; c < kPer - 1; ++c)
+                if (c < inside[p]) to[c] = v[c];
+            }
+          }
+        }
       }
       __builtin_amdgcn_sched_barrier(0);  // registers: no more than 16 tokens at a time
     }
@@ -682,9 +714,11 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
 #pragma unroll
       for (int j = 0; j < kNT; ++j) Pin(acc[i][j]);
     int8_t* const mine = lds + kStages * kStageBytes + wave * (kNT * 1024);
-    if (!a.vector_rows) FinishWave<T, false, true>(a, tile, wm * (BM / kWM), wn * (BN / kWN), mine, acc);
-    else if (a.residual) FinishWave<T, true, true>(a, tile, wm * (BM / kWM), wn * (BN / kWN), mine, acc);
-    else FinishWave<T, true, false>(a, tile, wm * (BM / kWM), wn * (BN / kWN), mine, acc);
+    const int m = wm * (BM / kWM), n = wn * (BN / kWN);
+    if (!a.vector_rows) FinishWave<T, kAny, true>(a, tile, m, n, mine, acc);
+    else if (!a.line_rows) FinishWave<T, kPieces, true>(a, tile, m, n, mine, acc);
+    else if (a.residual) FinishWave<T, kLines, true>(a, tile, m, n, mine, acc);
+    else FinishWave<T, kLines, false>(a, tile, m, n, mine, acc);
     tile.at += gridDim.x >> 3;
     tile.Place<BM, BN>(a, tiles);
     if (tile.rows == 0) break;
@@ -693,15 +727,25 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
 }
 
 // Rows that do not start at multiples of 16 bytes are copied to rows that do, zeros behind them: the DMA moves whole
-// 16-byte pieces.  x's rows come first, w's behind them.
+// 16-byte pieces.  x's rows come first, w's behind them.  A thread has kPadPieces pieces on their way at a time.
+constexpr int kPadPieces = 4;
+
 __global__ __launch_bounds__(256) void PadKernel(LinearArgs a, int8_t* __restrict__ to, int pieces, int pitch) {
   const long long count = (a.m + a.n) * pieces;
-  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<long long>(gridDim.x) * 256) {
+  const long long first = static_cast<long long>(blockIdx.x) * (256 * kPadPieces) + threadIdx.x;
+  int4v piece[kPadPieces];
+  int8_t* at[kPadPieces];
+  int k[kPadPieces];
+#pragma unroll
+  for (int j = 0; j < kPadPieces; ++j) {
+    const long long i = min(first + j * 256, count - 1);  // the last one is written by several threads, with the same bytes
     const long long row = count >> 31 ? i / pieces : static_cast<unsigned>(i) / static_cast<unsigned>(pieces);
-    const int k = static_cast<int>(i - row * pieces) * 16;
-    const int8_t* from = row < a.m ? a.x + row * a.x_stride : a.w + (row - a.m) * a.w_stride;
-    *reinterpret_cast<int4v*>(to + row * pitch + k) = LoadTail(from, k, a.k);
+    k[j] = static_cast<int>(i - row * pieces) * 16;
+    at[j] = to + row * pitch + k[j];
+    piece[j] = RequestPiece(row < a.m ? a.x + row * a.x_stride : a.w + (row - a.m) * a.w_stride, k[j], a.k);
   }
+#pragma unroll
+  for (int j = 0; j < kPadPieces; ++j) *reinterpret_cast<int4v*>(at[j]) = PieceOf(piece[j], k[j], a.k);
 }
 
 int Status() {
@@ -836,9 +880,10 @@ int Launch(LinearArgs a, void* workspace, hipStream_t st) {
     if (!workspace) return -4;
     const int row = PaddedRow(a.k);
     const int pieces = (a.k + 15) / 16;
-    const long long blocks = ((a.m + a.n) * pieces + 255) / 256;
-    hipLaunchKernelGGL(PadKernel, dim3(static_cast<unsigned>(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, a,
-                       static_cast<int8_t*>(workspace), pieces, row);
+    const long long blocks = ((a.m + a.n) * pieces + 256 * kPadPieces - 1) / (256 * kPadPieces);
+    if (blocks >= 1 << 24) return -3;
+    hipLaunchKernelGGL(PadKernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a, static_cast<int8_t*>(workspace), pieces,
+                       row);
     a.x = static_cast<const int8_t*>(workspace);
     a.w = a.x + a.m * row;
     a.x_stride = a.w_stride = row;
@@ -868,13 +913,15 @@ int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, co
   if (!x || !x_scale || !w || !w_scale || !y || m <= 0 || n <= 0 || k <= 0) return -1;
   if (dtype != tca::kF32 && dtype != tca::kF16 && dtype != tca::kBF16) return -2;
   if (k > 131071 || (reinterpret_cast<uintptr_t>(workspace) & 15)) return -3;
+  const int size = dtype == tca::kF32 ? 4 : 2;
   const bool vector_rows = ((reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias) |
-                             reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 15) == 0 &&
-                           ((n | y_stride | (residual ? residual_stride : 0)) & 7) == 0;
+                             reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual) |
+                             static_cast<uintptr_t>((n | y_stride | (residual ? residual_stride : 0)) * size)) & 15) == 0;
+  const bool line_rows = ((reinterpret_cast<uintptr_t>(y) | static_cast<uintptr_t>(y_stride * size)) & 127) == 0;
   const LinearArgs a{static_cast<const int8_t*>(x), static_cast<const float*>(x_scale), static_cast<const int8_t*>(w),
                      static_cast<const float*>(w_scale), bias, residual, y, m, n, x_stride, w_stride,
                      residual ? residual_stride : 0, y_stride, static_cast<int>(k), dtype,
-                     m <= 16 && n * k >= kPassing, vector_rows};
+                     m <= 16 && n * k >= kPassing, vector_rows, line_rows};
   return Launch(a, workspace, static_cast<hipStream_t>(stream));
 }
 
