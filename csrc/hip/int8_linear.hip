@@ -827,56 +827,97 @@ constexpr long long kPassing = 128ll << 20;
 // Descriptors hold 32-bit offsets: 256 rows of a tile have to stay below 2^30 bytes.
 constexpr long long kMostStride = 1 << 20;
 
-// Copying the operands to aligned rows costs their bytes twice and a launch, and lets the tile kernel in: 26 instead of 61
-// us at 1000 x 4000 x 2001, but 12.1 both ways at 1000 x 1000 x 1001 and 18 instead of 14 at 2000 x 200 x 3001.
-bool Pads(long long m, long long n) { return m > 64 && n >= 256 && m * n > (1 << 20); }
-
 // Rows at whole lines: at other multiples of 16 every request of a line touches two (3999 x 4016 apart, 48 instead of 40 us).
 int PaddedRow(long long k) { return static_cast<int>((k + 127) / 128 * 128); }
 
-// The largest tile that leaves no more than a quarter of the 256 CUs idle, else the smallest: what a CU takes in per
-// output falls with the tile's sides, but half the CUs take in half the bytes per second.
-template <typename T>
-int LaunchAligned(const LinearArgs& a, hipStream_t st) {
-  auto fills = [&](long long bm, long long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) >= 192; };
-  if (a.m > 64) {
-    if (fills(256, 256)) return LaunchTile<T, 256, 256, 2, 2, 2, 1>(a, st);
-    if (fills(256, 128)) return LaunchTile<T, 256, 128, 2, 2, 3, 1>(a, st);
-    if (fills(128, 128)) return LaunchTile<T, 128, 128, 2, 2, 2, 2>(a, st);
-  }
-  if (a.m > 32) {
-    if (fills(64, 128)) return LaunchTile<T, 64, 128, 2, 2, 2, 2>(a, st);
-    if (fills(64, 64)) return LaunchTile<T, 64, 64, 2, 2, 2, 4>(a, st);
-  }
-  // From here on k is split over the waves of a block; the more of them the longer it is, each has a few steps of 128.
-  const bool longer = a.k > 2048;
-  if (a.m > 16) {
-    if (fills(32, 64)) return longer ? LaunchSplitDma<2, 4, 8, 1>(a, st) : LaunchSplitDma<2, 4, 4, 1>(a, st);
-    if (fills(32, 32)) return longer ? LaunchSplitDma<2, 2, 4, 2>(a, st) : LaunchSplitDma<2, 2, 2, 2>(a, st);
-    if (longer && fills(32, 16)) return LaunchSplitDma<2, 1, 8, 2>(a, st);
-  } else if (fills(16, 64)) {
-    return LaunchSplitDma<1, 4, 8, 1>(a, st);
-  }
-  if (fills(16, 32)) return longer ? LaunchSplitDma<1, 2, 8, 2>(a, st) : LaunchSplitDma<1, 2, 2, 2>(a, st);
-  if (a.k > 8192) return LaunchSplitDma<1, 1, 16, 2>(a, st);
-  return longer ? LaunchSplitDma<1, 1, 8, 2>(a, st) : LaunchSplitDma<1, 1, 4, 2>(a, st);
+// Which kernel takes a product: the one whose time comes out least.  A CU has `tiles` of them to work through, `blocks` at a
+// time.  One alone needs step_alone for each 128 k (of each of `waves` parts of k) and end_alone besides; with all `blocks`
+// of a CU at work, each of them takes its step and end from what they share.  What an unaligned row adds to the ends is
+// `odd`.  In us, fitted to the times of 750 products of random sizes (m to 8192, n and k to 16384; 550 for unaligned rows):
+// the choice is on average 1.7% behind the fastest kernel here, where "the largest tile that fills three quarters of the
+// CUs" was 9% behind (6177 x 8769 x 128: 83 -> 54 us; 1985 x 1216 x 7488: 41 -> 32; 2213 x 6330 x 384: 30 -> 22).
+struct Way {
+  int rows, columns, waves, blocks;
+  float step_alone, end_alone, step, end, odd;
+};
+
+constexpr float kLaunch = 2.f;
+
+float Estimate(const Way& w, long long m, long long n, long long k) {
+  const long long tiles = (((m + w.rows - 1) / w.rows) * ((n + w.columns - 1) / w.columns) + 255) / 256;  // of a CU
+  const float steps = static_cast<float>(((k + kStep - 1) / kStep + w.waves - 1) / w.waves);
+  const float odd = n % 8 ? 1.f + w.odd : 1.f;
+  const float alone = static_cast<float>((tiles + w.blocks - 1) / w.blocks) * (steps * w.step_alone + w.end_alone * odd);
+  const float shared = static_cast<float>(tiles) * (steps * w.step + w.end * odd);
+  return kLaunch + (alone > shared ? alone : shared);
 }
 
-int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
-  auto fills = [&](long long bm, long long bn) { return ((a.m + bm - 1) / bm) * ((a.n + bn - 1) / bn) >= 192; };
-  if (a.m > 16) {
-    if (fills(32, 64)) return LaunchSplitAny<2, 4, 4>(a, st);
-    if (fills(32, 32)) return a.k > 1024 ? LaunchSplitAny<2, 2, 8>(a, st) : LaunchSplitAny<2, 2, 4>(a, st);
-  } else if (fills(16, 64)) {
-    return LaunchSplitAny<1, 4, 8>(a, st);
+template <int kCount>
+int Fastest(const Way (&ways)[kCount], long long m, long long n, long long k, float* time = nullptr) {
+  int best = 0;
+  float least = 0.f;
+  for (int i = 0; i < kCount; ++i) {
+    const float t = Estimate(ways[i], m, n, k);
+    if (i == 0 || t < least) {
+      best = i;
+      least = t;
+    }
   }
-  if (fills(16, 32)) return LaunchSplitAny<1, 2, 8>(a, st);
-  return a.k > 1024 ? LaunchSplitAny<1, 1, 16>(a, st) : LaunchSplitAny<1, 1, 4>(a, st);
+  if (time) *time = least;
+  return best;
+}
+
+constexpr Way kAligned[] = {{256, 256, 1, 1, 1.14f, 7.24f, 0.11f, 0.80f, 0.80f}, {256, 128, 1, 1, 0.74f, 4.30f, 0.30f, 0.80f, 0.72f},
+                            {128, 128, 1, 2, 0.35f, 2.92f, 0.47f, 1.49f, 0.56f}, {64, 128, 1, 2, 0.34f, 1.89f, 0.33f, 1.02f, 0.53f},
+                            {64, 64, 1, 4, 0.27f, 1.48f, 0.21f, 0.62f, 0.40f},   {32, 64, 8, 1, 1.40f, 1.32f, 0.48f, 0.80f, 0.12f},
+                            {32, 32, 4, 2, 0.31f, 1.38f, 0.44f, 0.91f, 0.25f},   {32, 16, 4, 3, 0.21f, 1.05f, 0.29f, 0.60f, 0.41f},
+                            {16, 32, 4, 3, 0.25f, 0.95f, 0.31f, 0.56f, 0.49f},   {16, 16, 8, 2, 0.32f, 0.85f, 0.39f, 0.62f, 0.56f},
+                            {16, 16, 4, 5, 0.18f, 0.76f, 0.23f, 0.34f, 0.68f},   {16, 16, 2, 10, 0.17f, 0.76f, 0.13f, 0.19f, 0.66f}};
+
+template <typename T>
+int LaunchAligned(const LinearArgs& a, hipStream_t st) {
+  switch (Fastest(kAligned, a.m, a.n, a.k)) {
+    case 0: return LaunchTile<T, 256, 256, 2, 2, 2, 1>(a, st);
+    case 1: return LaunchTile<T, 256, 128, 2, 2, 3, 1>(a, st);
+    case 2: return LaunchTile<T, 128, 128, 2, 2, 2, 2>(a, st);
+    case 3: return LaunchTile<T, 64, 128, 2, 2, 2, 2>(a, st);
+    case 4: return LaunchTile<T, 64, 64, 2, 2, 2, 4>(a, st);
+    case 5: return LaunchSplitDma<2, 4, 8, 1>(a, st);
+    case 6: return LaunchSplitDma<2, 2, 4, 2>(a, st);
+    case 7: return LaunchSplitDma<2, 1, 4, 2>(a, st);
+    case 8: return LaunchSplitDma<1, 2, 4, 2>(a, st);
+    case 9: return LaunchSplitDma<1, 1, 8, 2>(a, st);
+    case 10: return LaunchSplitDma<1, 1, 4, 2>(a, st);
+    default: return LaunchSplitDma<1, 1, 2, 2>(a, st);
+  }
+}
+
+constexpr Way kUnaligned[] = {{32, 64, 4, 3, 1.27f, 3.57f, 1.22f, 1.92f, 0.25f}, {32, 32, 8, 2, 1.71f, 1.25f, 1.50f, 0.69f, 0.38f},
+                              {32, 32, 4, 4, 0.82f, 2.12f, 0.79f, 0.55f, 0.25f}, {16, 32, 4, 4, 0.60f, 1.58f, 0.59f, 0.40f, 0.33f},
+                              {16, 16, 16, 1, 1.57f, 0.31f, 0.30f, 0.80f, 1.46f}, {16, 16, 4, 4, 0.45f, 1.10f, 0.41f, 0.11f, 0.46f}};
+
+int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
+  switch (Fastest(kUnaligned, a.m, a.n, a.k)) {
+    case 0: return LaunchSplitAny<2, 4, 4>(a, st);
+    case 1: return LaunchSplitAny<2, 2, 8>(a, st);
+    case 2: return LaunchSplitAny<2, 2, 4>(a, st);
+    case 3: return LaunchSplitAny<1, 2, 4>(a, st);
+    case 4: return LaunchSplitAny<1, 1, 16>(a, st);
+    default: return LaunchSplitAny<1, 1, 4>(a, st);
+  }
+}
+
+// Copying the operands to aligned rows lets the DMA and the large tiles in; it costs a launch and the operands' bytes twice.
+bool Pads(long long m, long long n, long long k) {
+  float aligned, unaligned;
+  Fastest(kAligned, m, n, k, &aligned);
+  Fastest(kUnaligned, m, n, k, &unaligned);
+  return aligned + 3.2f + 4.3e-7f * static_cast<float>(m + n) * static_cast<float>(k) < unaligned;
 }
 
 int Launch(LinearArgs a, void* workspace, hipStream_t st) {
   if (!Aligned(a.x, a.w, a.x_stride, a.w_stride, a.k)) {
-    if (!Pads(a.m, a.n)) return LaunchUnaligned(a, st);
+    if (!Pads(a.m, a.n, a.k)) return LaunchUnaligned(a, st);
     if (!workspace) return -4;
     const int row = PaddedRow(a.k);
     const int pieces = (a.k + 15) / 16;
@@ -902,7 +943,7 @@ extern "C" {
 // Bytes of workspace (at a multiple of 16) that a launch with these operands needs; mostly 0.
 long long tca_int8_linear_workspace_bytes(const void* x, const void* w, long long m, long long n, long long k, long long x_stride,
                                           long long w_stride) {
-  if (m <= 0 || n <= 0 || k <= 0 || Aligned(x, w, x_stride, w_stride, k) || !Pads(m, n)) return 0;
+  if (m <= 0 || n <= 0 || k <= 0 || Aligned(x, w, x_stride, w_stride, k) || !Pads(m, n, k)) return 0;
   return (m + n) * PaddedRow(k);
 }
 
