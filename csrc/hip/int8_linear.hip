@@ -832,16 +832,15 @@ int PaddedRow(long long k) { return static_cast<int>((k + 127) / 128 * 128); }
 
 // Which kernel takes a product: the one whose time comes out least.  A CU has `tiles` of them to work through, `blocks` at a
 // time.  One alone needs step_alone for each 128 k (of each of `waves` parts of k) and end_alone besides; with all `blocks`
-// of a CU at work, each of them takes its step and end from what they share.  What an unaligned row adds to the ends is
-// `odd`.  In us, fitted to the times of 1100 products of random sizes (m to 8192, n and k to 16384; 550 for unaligned rows):
-// the choice is on average 1.6% behind the fastest kernel here, where "the largest tile that fills three quarters of the
-// CUs" was 9% behind (6177 x 8769 x 128: 83 -> 54 us; 1985 x 1216 x 7488: 41 -> 32; 2213 x 6330 x 384: 30 -> 22).
+// of a CU at work, each of them takes its step and end from what they share.  Outputs at odd addresses lengthen the ends by
+// `odd`.  In us, without the launch and apart from the time of the bytes from memory, which is the same for all.  Fitted to
+// the times of 1700 products of random sizes (m to 8192, n and k to 16384; 550 for rows at any address): the choice is on
+// average 1.9% behind the fastest kernel here, where "the largest tile that fills three quarters of the CUs" was 9% behind
+// (6177 x 8769 x 128: 83 -> 54 us; 1985 x 1216 x 7488: 41 -> 32; 2213 x 6330 x 384: 30 -> 22).
 struct Way {
   int rows, columns, waves, blocks;
   float step_alone, end_alone, step, end, odd;
 };
-
-constexpr float kLaunch = 2.f;
 
 float Estimate(const Way& w, long long m, long long n, long long k) {
   const long long tiles = (((m + w.rows - 1) / w.rows) * ((n + w.columns - 1) / w.columns) + 255) / 256;  // of a CU
@@ -849,7 +848,7 @@ float Estimate(const Way& w, long long m, long long n, long long k) {
   const float odd = n % 8 ? 1.f + w.odd : 1.f;
   const float alone = static_cast<float>((tiles + w.blocks - 1) / w.blocks) * (steps * w.step_alone + w.end_alone * odd);
   const float shared = static_cast<float>(tiles) * (steps * w.step + w.end * odd);
-  return kLaunch + (alone > shared ? alone : shared);
+  return alone > shared ? alone : shared;
 }
 
 // Tiles at least half of whose rows would be empty are left out: few rows are bound by memory, where estimates meet.
@@ -869,13 +868,13 @@ int Fastest(const Way (&ways)[kCount], long long m, long long n, long long k, fl
   return best;
 }
 
-constexpr Way kAligned[] = {{256, 256, 1, 1, 1.15f, 7.29f, 0.13f, 0.80f, 0.78f}, {256, 128, 1, 1, 0.74f, 4.43f, 0.32f, 0.80f, 0.70f},
-                            {128, 128, 1, 2, 0.39f, 2.85f, 0.46f, 1.55f, 0.57f}, {64, 128, 1, 2, 0.34f, 1.90f, 0.32f, 1.06f, 0.53f},
-                            {64, 64, 1, 4, 0.27f, 1.49f, 0.21f, 0.64f, 0.38f},   {32, 64, 8, 1, 1.40f, 1.33f, 0.48f, 0.80f, 0.11f},
-                            {32, 32, 4, 2, 0.32f, 1.37f, 0.44f, 0.90f, 0.25f},   {32, 16, 4, 3, 0.20f, 1.06f, 0.29f, 0.59f, 0.41f},
-                            {16, 32, 4, 3, 0.26f, 0.97f, 0.36f, 0.54f, 0.42f},   {16, 32, 2, 6, 0.25f, 0.87f, 0.22f, 0.31f, 0.50f},
-                            {16, 16, 8, 2, 0.32f, 0.90f, 0.44f, 0.60f, 0.47f},   {16, 16, 4, 5, 0.21f, 0.75f, 0.25f, 0.34f, 0.62f},
-                            {16, 16, 2, 10, 0.19f, 0.74f, 0.14f, 0.19f, 0.62f}};
+constexpr Way kAligned[] = {{256, 256, 1, 1, 1.16f, 6.96f, 0.18f, 0.80f, 0.86f}, {256, 128, 1, 1, 0.73f, 4.34f, 0.30f, 0.80f, 0.72f},
+                            {128, 128, 1, 2, 0.39f, 2.78f, 0.46f, 1.43f, 0.60f}, {64, 128, 1, 2, 0.34f, 1.89f, 0.32f, 1.02f, 0.54f},
+                            {64, 64, 1, 4, 0.26f, 1.50f, 0.20f, 0.62f, 0.39f},   {32, 64, 8, 1, 1.37f, 1.34f, 0.13f, 0.80f, 0.12f},
+                            {32, 32, 4, 2, 0.31f, 1.37f, 0.42f, 0.90f, 0.26f},   {32, 16, 4, 3, 0.20f, 1.05f, 0.28f, 0.58f, 0.43f},
+                            {16, 64, 8, 2, 0.84f, 1.03f, 0.96f, 0.68f, 0.38f},   {16, 32, 4, 3, 0.24f, 0.97f, 0.29f, 0.57f, 0.48f},
+                            {16, 32, 2, 6, 0.23f, 0.90f, 0.16f, 0.37f, 0.50f},   {16, 16, 8, 2, 0.30f, 0.90f, 0.34f, 0.69f, 0.48f},
+                            {16, 16, 4, 5, 0.20f, 0.76f, 0.18f, 0.40f, 0.62f},   {16, 16, 2, 10, 0.20f, 0.73f, 0.10f, 0.24f, 0.60f}};
 
 template <typename T>
 int LaunchAligned(const LinearArgs& a, hipStream_t st) {
@@ -888,10 +887,11 @@ int LaunchAligned(const LinearArgs& a, hipStream_t st) {
     case 5: return LaunchSplitDma<2, 4, 8, 1>(a, st);
     case 6: return LaunchSplitDma<2, 2, 4, 2>(a, st);
     case 7: return LaunchSplitDma<2, 1, 4, 2>(a, st);
-    case 8: return LaunchSplitDma<1, 2, 4, 2>(a, st);
-    case 9: return LaunchSplitDma<1, 2, 2, 2>(a, st);
-    case 10: return LaunchSplitDma<1, 1, 8, 2>(a, st);
-    case 11: return LaunchSplitDma<1, 1, 4, 2>(a, st);
+    case 8: return LaunchSplitDma<1, 4, 8, 1>(a, st);
+    case 9: return LaunchSplitDma<1, 2, 4, 2>(a, st);
+    case 10: return LaunchSplitDma<1, 2, 2, 2>(a, st);
+    case 11: return LaunchSplitDma<1, 1, 8, 2>(a, st);
+    case 12: return LaunchSplitDma<1, 1, 4, 2>(a, st);
     default: return LaunchSplitDma<1, 1, 2, 2>(a, st);
   }
 }
