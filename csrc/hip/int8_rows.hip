@@ -101,7 +101,8 @@ __device__ __forceinline__ void Values(Chunk<T> c, int first, int width, float (
 
 // N bytes to any address, by non-temporal stores: what a kernel writes does not push out what it and its neighbours are
 // still to read (norm and read-back of 16384 x 8192: 240 -> 229 us, the norm alone of 2048 x 8192 28.8 -> 22.4; a reader
-// that follows at once finds small results no later, 36.3 and 36.4 us for that norm and its read-back).
+// that follows at once finds small results no later, 36.3 and 36.4 us for that norm and its read-back).  Not where a lane
+// has 32 bytes: each of its stores leaves gaps between the lanes, to be filled by the next, and that needs the caches.
 template <int N>
 __device__ __forceinline__ void StoreBytes(void* to, const void* from) {
   using Word = __attribute__((ext_vector_type(N >= 16 ? 4 : 2))) unsigned;
@@ -110,20 +111,22 @@ __device__ __forceinline__ void StoreBytes(void* to, const void* from) {
   for (int i = 0; i < N / static_cast<int>(sizeof(Word)); ++i) {
     Word w;
     __builtin_memcpy(&w, static_cast<const char*>(from) + i * sizeof(Word), sizeof(Word));
-    __builtin_nontemporal_store(w, reinterpret_cast<AnyAddress*>(static_cast<char*>(to) + i * sizeof(Word)));
+    AnyAddress* const at = reinterpret_cast<AnyAddress*>(static_cast<char*>(to) + i * sizeof(Word));
+    if constexpr (N == sizeof(Word)) __builtin_nontemporal_store(w, at);
+    else *at = w;
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void StoreChunk(T* row, int first, int width, const float (&v)[kVec]) {
-  T t[kVec];
+template <typename T, int kCount>
+__device__ __forceinline__ void StoreChunk(T* row, int first, int width, const float (&v)[kCount]) {
+  T t[kCount];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) t[i] = FromFloat<T>(v[i]);
-  if (first + kVec <= width) {
+  for (int i = 0; i < kCount; ++i) t[i] = FromFloat<T>(v[i]);
+  if (first + kCount <= width) {
     StoreBytes<sizeof(t)>(row + first, t);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i)
+    for (int i = 0; i < kCount; ++i)
       if (first + i < width) row[first + i] = t[i];
   }
 }
@@ -433,29 +436,31 @@ __global__ __launch_bounds__(1024) void LongRowsKernel(RowArgs a) {
   }
 }
 
-// out[row][k] = round(q[row][k] * scale[row]); one chunk of eight per thread
+// out[row][k] = round(q[row][k] * scale[row]); a thread has 16 bytes of results, so that a wave's store fills whole lines
+// (fp32 of 8192 x 8192: with 32 bytes a thread 98 us, or 60 through the caches).
 template <typename T>
 __global__ __launch_bounds__(256) void DequantizeKernel(const int8_t* __restrict__ q, const float* __restrict__ scale,
                                                         T* __restrict__ out, long long rows, int width,
                                                         int chunks_per_row, long long q_stride, long long out_stride) {
+  constexpr int kCount = 16 / sizeof(T);
   const long long chunks = rows * chunks_per_row;
   for (long long at = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; at < chunks;
        at += static_cast<long long>(gridDim.x) * 256) {
     const long long row = chunks >> 31 ? at / chunks_per_row
                                        : static_cast<unsigned>(at) / static_cast<unsigned>(chunks_per_row);
-    const int first = static_cast<int>(at - row * chunks_per_row) * kVec;
+    const int first = static_cast<int>(at - row * chunks_per_row) * kCount;
     const int8_t* src = q + row * q_stride + first;
     const float s = scale[row];
     uint64_t packed = 0;
-    if (first + kVec <= width) {
-      __builtin_memcpy(&packed, src, sizeof(packed));
+    if (first + kCount <= width) {
+      __builtin_memcpy(&packed, src, kCount);
     } else {
       for (int i = 0; first + i < width; ++i)
         packed |= static_cast<uint64_t>(static_cast<uint8_t>(src[i])) << (8 * i);
     }
-    float v[kVec];
+    float v[kCount];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) v[i] = static_cast<float>(static_cast<int8_t>(packed >> (8 * i))) * s;
+    for (int i = 0; i < kCount; ++i) v[i] = static_cast<float>(static_cast<int8_t>(packed >> (8 * i))) * s;
     StoreChunk(out + row * out_stride, first, width, v);
   }
 }
@@ -573,7 +578,8 @@ int tca_int8_rms_norm_launch(const void* x, const void* residual, const void* we
 int tca_int8_dequantize_launch(const void* q, const void* scale, void* out, int dtype, long long rows, long long width,
                                long long q_stride, long long out_stride, void* stream) {
   if (!q || !scale || !out || BadExtent(rows, width)) return -1;
-  const int chunks_per_row = static_cast<int>((width + kVec - 1) / kVec);
+  const int count = dtype == tca::kF32 ? 4 : 8;  // values in 16 bytes of results
+  const int chunks_per_row = static_cast<int>((width + count - 1) / count);
   const long long blocks = (rows * chunks_per_row + 255) / 256;
   const dim3 grid(static_cast<unsigned>(blocks < (1ll << 23) ? blocks : 1ll << 23));  // the kernel takes the rest in turns
   const int8_t* src = static_cast<const int8_t*>(q);
