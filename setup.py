@@ -35,7 +35,7 @@ class BuildWithNative(build_py):
 
             targets = ["core", "pyext"]
             if os.environ.get("TCA_SKIP_HIP_BUILD") != "1":
-                targets.append("hip")
+                targets += ["hip", "torch"]
             _build.build(targets)
         super().run()
 

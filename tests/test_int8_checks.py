@@ -133,3 +133,16 @@ def test_pending_negations_are_refused():
                  lambda: _linear(x_scale=x[0, :3]), lambda: _linear(weight_scale=x[0, :4])):
         with pytest.raises(ValueError, match="negation"):
             call()
+
+
+def test_without_the_extension(monkeypatch):
+    """An extension that does not load costs a warning and time, not the operators."""
+    def missing():
+        raise ImportError("built for another torch")
+
+    monkeypatch.setattr(int8, "_plain", None)
+    monkeypatch.setattr(int8._native, "torch_ops", missing)
+    with pytest.warns(RuntimeWarning, match="built for another torch"), pytest.raises(ValueError, match="CUDA"):
+        int8.quantize_int8(_x(2, 8))
+    with pytest.raises(ValueError, match="CUDA"):  # and no second warning
+        int8.quantize_int8(_x(2, 8))

@@ -29,6 +29,9 @@ instead of a number.  The reference has no model code (its models run in the ser
 
 from __future__ import annotations
 
+import subprocess
+import warnings
+
 import torch
 
 from .. import _native
@@ -45,9 +48,22 @@ _CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _plain = None
 
 
+class _General:
+    """In the place of an extension that this torch does not load and that cannot be built here: no call is plain."""
+
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
 def _load_plain():
     global _plain
-    _plain = _native.torch_ops()
+    lib()  # without the kernels there is no way to go on
+    try:
+        _plain = _native.torch_ops()
+    except (ImportError, FileNotFoundError, subprocess.CalledProcessError) as e:
+        warnings.warn(f"8-bit operators: calls take their slower way in Python, the extension is not there ({e})",
+                      RuntimeWarning, stacklevel=3)
+        _plain = _General()
     return _plain
 
 
