@@ -11,14 +11,19 @@
 // to lanes gives the same sum.  The weight is the MFMA's first operand: a lane then holds four consecutive outputs of
 // one token.
 //
-// SplitDmaKernel  the waves of a block share the k axis of one small output tile: every wave multiplies its own k steps of
-//              128, the sums meet in LDS.  SplitAnyKernel: the same for rows that do not start at multiples of 16 bytes.
-// TileKernel   large products: 256 x 256 (or 128 x 128) outputs per block of four waves, operands through a ring of LDS
-//              stages filled by DMA.  8192 x 8192 x 8192 to bf16: 408 us (2.69 POP/s), 462 us with a residual.  What
-//              bounds it is the card's power: on zeros, where nothing toggles, the same call takes 303 us.  One wave per
-//              SIMD with 128 x 128 outputs reads the fewest bytes from LDS per product and wins over two waves with
-//              128 x 64 (420 us); products of 16 x 16 x 64 touch the accumulators half as often per operation as those of
-//              32 x 32 x 32 and win although they issue twice as often (443 against 476 us at the same stage of tuning).
+// SplitDmaKernel  few tokens or small outputs: the waves of a block share the k axis of one small output tile, every wave
+//              multiplies its own k steps of 128 from a ring of its own in LDS, filled by DMA; the sums meet in LDS.  Bound
+//              by memory: 16 x 32768 x 4096 in 25 to 28 us (4.8 to 5.4 TB/s), 1 x 4096 x 4096 in 4.5 us on the GPU.
+// SplitAnyKernel  the same for rows that do not start at multiples of 16 bytes, through registers.
+// TileKernel   large products: tiles of 64 x 64 to 256 x 256 outputs per block of four waves, operands through LDS stages
+//              filled by DMA.  8192 x 8192 x 8192 to bf16: 371 to 395 us on two cards (2.8 to 3.0 POP/s), 382 to 411 with a
+//              residual.  What bounds it is the card's power: on zeros, where nothing toggles, the same call took 296 us (312
+//              with a residual) on the faster one, and its products alone, fed from registers, 293 us on real values and
+//              259 on zeros.  One wave per SIMD with 128 x 128 outputs reads the fewest bytes from LDS per product and won
+//              over two waves with 128 x 64 (408 against 420 us at an earlier stage of tuning); products of 16 x 16 x 64
+//              touch the accumulators half as often per operation as those of 32 x 32 x 32 and won although they issue
+//              twice as often (443 against 476 us, earlier still).
+// Every launch is one kernel; a large product whose rows start anywhere is two (PadKernel first).
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -827,7 +832,8 @@ constexpr long long kPassing = 128ll << 20;
 // Descriptors hold 32-bit offsets: 256 rows of a tile have to stay below 2^30 bytes.
 constexpr long long kMostStride = 1 << 20;
 
-// Rows at whole lines: at other multiples of 16 every request of a line touches two (3999 x 4016 apart, 48 instead of 40 us).
+// Rows at whole lines: at other multiples of 16 every request of a line touches two (2048 x 4096 x 4096: 48.5 us with rows
+// 16 bytes further apart than the lines, 40.4 at whole lines).
 int PaddedRow(long long k) { return static_cast<int>((k + 127) / 128 * 128); }
 
 // Which kernel takes a product: the one whose time comes out least.  A CU has `tiles` of them to work through, `blocks` at a
@@ -876,9 +882,14 @@ constexpr Way kAligned[] = {{256, 256, 1, 1, 1.16f, 6.96f, 0.18f, 0.80f, 0.86f},
                             {16, 32, 2, 6, 0.23f, 0.90f, 0.16f, 0.37f, 0.50f},   {16, 16, 8, 2, 0.30f, 0.90f, 0.34f, 0.69f, 0.48f},
                             {16, 16, 4, 5, 0.20f, 0.76f, 0.18f, 0.40f, 0.62f},   {16, 16, 2, 10, 0.20f, 0.73f, 0.10f, 0.24f, 0.60f}};
 
+// A large weight for up to eight tokens is bound by memory alone, and what differs is how the rows that are asked for at a
+// time fall on its channels, which the estimates do not know: narrow tiles of 16 rows do best where rows are a power of two
+// apart (1 x 16384 x 8192: 22.9 us, where 32 rows take 29.1) and as well as others elsewhere.
+constexpr long long kStreams = 64ll << 20;
+
 template <typename T>
 int LaunchAligned(const LinearArgs& a, hipStream_t st) {
-  switch (Fastest(kAligned, a.m, a.n, a.k)) {
+  switch (a.m <= 8 && a.n * a.k >= kStreams ? 12 : Fastest(kAligned, a.m, a.n, a.k)) {
     case 0: return LaunchTile<T, 256, 256, 2, 2, 2, 1>(a, st);
     case 1: return LaunchTile<T, 256, 128, 2, 2, 3, 1>(a, st);
     case 2: return LaunchTile<T, 128, 128, 2, 2, 2, 2>(a, st);
@@ -911,7 +922,8 @@ int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
   }
 }
 
-// Copying the operands to aligned rows lets the DMA and the large tiles in; it costs a launch and the operands' bytes twice.
+// Copying the operands to aligned rows lets the DMA and the large tiles in; it costs a launch and the operands' bytes twice
+// (3.2 us and 0.43 us per MB).  1756 x 1856 x 4199: 29 us copied, 88 as they are; 125 x 5248 x 2315: 19.2 and 16.4.
 bool Pads(long long m, long long n, long long k) {
   float aligned, unaligned;
   Fastest(kAligned, m, n, k, &aligned);

@@ -219,7 +219,8 @@ def _quantize(x, gated, out, scale):
 def quantize_int8(x, out=None, scale=None):
     """``(q int8 [..., K], scale fp32 [...])`` of ``x [..., K]``: with ``m`` the largest magnitude of a row, ``q`` is the
     integer nearest to ``127 x / m`` (ties to even, decided exactly) and ``scale = m / 127`` (one step less where
-    ``127 * scale`` would leave fp32's range).  A row of zeros has the scale 0.  ``out`` and ``scale`` may be destinations of the results' shapes."""
+    ``127 * scale`` would leave fp32's range).  A row of zeros has the scale 0.  ``out`` and ``scale`` may be
+    destinations of the results' shapes."""
     if out is None and scale is None:
         made = (_plain or _load_plain()).quantize(x, False)
         if made is not None:
