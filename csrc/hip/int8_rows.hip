@@ -474,16 +474,21 @@ int Status() {
 constexpr long long kMostRows = 1ll << 21;
 
 // Few rows: as many threads as a row has chunks, every chunk's way from memory at the same time (8 rows of 8192 bf16: 5.0
-// us with one chunk per thread, 7.0 with four).  Many rows fill the CUs anyway, and four chunks per thread keep more bytes
-// on their way in fewer waves (16384 rows: 81 us with four, 135 with one).  Norms of fp32 rows hold three fp32 inputs per
-// value: two chunks are what the registers of 1024 threads hold.
+// us with one chunk per thread, 7.0 with four).  Many rows fill the CUs anyway, and what counts is the bytes that a thread
+// has on their way: 64 do best, 32 where each CU has few rows.  Times with one, two and four chunks per thread, bf16 from
+// memory: 16384 rows of 8192 quantised 120, 87 and 74 us (16 bytes of input a chunk), the norm with a residual 184, 169 and
+// 172, the gate 138, 125 and 122 (32 bytes); 2048 rows of 4096 10.6, 9.9 and 11.0; 16.0, 17.4 and 19.0; 12.3, 12.2 and 13.6.
+// Norms of fp32 rows hold three fp32 inputs per value: two chunks are what the registers of 1024 threads hold.
 template <typename T, typename W, int kMode>
 void LaunchRows(RowArgs a, hipStream_t stream) {
   constexpr bool kWide = sizeof(T) == 4 && (kMode == kNorm || kMode == kNormResidual);
   const int chunks = (a.width + kVec - 1) / kVec;
   const long long rows = a.rows;
   const int most = kWide ? 2 : 4;
-  int per_thread = rows >= 2048 && chunks >= 512 ? most : 1;
+  constexpr int kInputs = kMode == kGate || kMode == kNormResidual ? 2 : 1;  // the norm's weight stays in the caches
+  const int bytes = rows >= 4096 ? 64 : 32;
+  int per_thread = rows >= 1024 && chunks >= 512 ? bytes / (kInputs * kVec * static_cast<int>(sizeof(T))) : 1;
+  per_thread = per_thread < 1 ? 1 : per_thread < most ? per_thread : most;
   while (per_thread < most && chunks > per_thread * 1024) per_thread *= 2;
   const dim3 threads(((chunks + per_thread - 1) / per_thread + 63) / 64 * 64);
   for (; a.first_row < rows; a.first_row += kMostRows) {
