@@ -715,3 +715,12 @@ def test_parameters_without_gradients():
         assert torch.equal(a, b) and not a.requires_grad
     frozen = torch.nn.Parameter(x.detach(), requires_grad=False)
     assert torch.equal(int8.quantize_int8(frozen)[0], int8.quantize_int8(x.detach())[0])
+
+
+def test_in_inference_mode():
+    """Results are what any operator's are there, on the extension's way and on the general one."""
+    x = _values(5, 64, torch.float16).cuda()
+    with torch.inference_mode():
+        for t in (*int8.quantize_int8(x), *int8.quantize_int8(x[:, 1:])):
+            assert t.is_inference()
+    assert not int8.quantize_int8(x)[0].is_inference()

@@ -102,7 +102,7 @@ def build_torch(force=False):
                          "-isystem", home / "include", "-isystem",
                          home / "include" / "torch" / "csrc" / "api" / "include", "-isystem", ROCM / "include",
                          "-isystem", sysconfig.get_paths()["include"], "-o", out, src, f"-L{home / 'lib'}",
-                         "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"], out)
+                         "-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"], out)
     return out
 
 
