@@ -61,9 +61,17 @@ __device__ __forceinline__ float ToFloat(_Float16 v) { return static_cast<float>
 __device__ __forceinline__ float ToFloat(Bf16 v) { return __uint_as_float(static_cast<unsigned>(v.bits) << 16); }
 template <typename T> __device__ __forceinline__ T FromFloat(float v);
 template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
-template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) { return static_cast<_Float16>(v); }
+template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) {
+  asm("" : "+v"(v));  // rounded to fp32 first, also where an instruction would round a product to fp16 at once
+  return static_cast<_Float16>(v);
+}
 template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
   return Bf16{__builtin_bit_cast(unsigned short, static_cast<__bf16>(v))};
+}
+
+// The same roundings in every kernel, so that a token's outputs do not depend on the others of its batch.
+__device__ __forceinline__ float Result(int sum, float scale, float bias, float residual) {
+  return __builtin_fmaf(static_cast<float>(sum), scale, bias) + residual;
 }
 
 // one lane's sums: outputs n .. n + 3 of token m
@@ -78,30 +86,19 @@ __device__ __forceinline__ void FinishFour(const LinearArgs& a, long long m, lon
   const float sx = a.x_scale[m];
   if (a.vector_rows) {  // n % 4 == 0, so all four are there
     const float4 sw = *reinterpret_cast<const float4*>(a.w_scale + n);
-    float v[4] = {static_cast<float>(sum[0]) * (sx * sw.x), static_cast<float>(sum[1]) * (sx * sw.y),
-                  static_cast<float>(sum[2]) * (sx * sw.z), static_cast<float>(sum[3]) * (sx * sw.w)};
-    if (a.bias) {
-      const Four b = *reinterpret_cast<const Four*>(bias);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += ToFloat(b.v[i]);
-    }
-    if (a.residual) {
-      const Four r = *reinterpret_cast<const Four*>(residual);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] += ToFloat(r.v[i]);
-    }
+    const float scale[4] = {sx * sw.x, sx * sw.y, sx * sw.z, sx * sw.w};
+    Four b{}, r{};
+    if (a.bias) b = *reinterpret_cast<const Four*>(bias);
+    if (a.residual) r = *reinterpret_cast<const Four*>(residual);
     Four out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) out.v[i] = FromFloat<T>(v[i]);
+    for (int i = 0; i < 4; ++i) out.v[i] = FromFloat<T>(Result(sum[i], scale[i], ToFloat(b.v[i]), ToFloat(r.v[i])));
     *reinterpret_cast<Four*>(y) = out;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (n + i >= a.n) return;
-      float v = static_cast<float>(sum[i]) * (sx * a.w_scale[n + i]);
-      if (a.bias) v += ToFloat(bias[i]);
-      if (a.residual) v += ToFloat(residual[i]);
-      y[i] = FromFloat<T>(v);
+      y[i] = FromFloat<T>(Result(sum[i], sx * a.w_scale[n + i], a.bias ? ToFloat(bias[i]) : 0.f, a.residual ? ToFloat(residual[i]) : 0.f));
     }
   }
 }
@@ -541,9 +538,10 @@ __device__ __forceinline__ void FinishWave(const LinearArgs& a, const TileCursor
             const int4v sum = *reinterpret_cast<const int4v*>(lds + from * (kNT * 64) + (at ^ (from & kTurnMask)) * 16);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              float f = static_cast<float>(sum[e]) * (sx[i][t] * sw[p * kPer + c + e]) + bias[p][c + e];
-              if constexpr (kResidual) f += r[i - first][t][p][c + e];
-              v[c + e] = FromFloat<T>(f);
+              const float scale = sx[i][t] * sw[p * kPer + c + e];
+              float residual_value = 0.f;
+              if constexpr (kResidual) residual_value = r[i - first][t][p][c + e];
+              v[c + e] = FromFloat<T>(Result(sum[e], scale, bias[p][c + e], residual_value));
             }
           }
           if constexpr (kRowsAt != kAny) {

@@ -50,7 +50,10 @@ __device__ __forceinline__ float ToFloat(Bf16 v) { return __uint_as_float(static
 
 template <typename T> __device__ __forceinline__ T FromFloat(float v);
 template <> __device__ __forceinline__ float FromFloat<float>(float v) { return v; }
-template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) { return static_cast<_Float16>(v); }
+template <> __device__ __forceinline__ _Float16 FromFloat<_Float16>(float v) {
+  asm("" : "+v"(v));  // rounded to fp32 first, also where an instruction would round a product to fp16 at once
+  return static_cast<_Float16>(v);
+}
 template <> __device__ __forceinline__ Bf16 FromFloat<Bf16>(float v) {
   return Bf16{__builtin_bit_cast(unsigned short, static_cast<__bf16>(v))};  // nearest, ties to even, NaN kept
 }

@@ -724,3 +724,36 @@ def test_in_inference_mode():
         for t in (*int8.quantize_int8(x), *int8.quantize_int8(x[:, 1:])):
             assert t.is_inference()
     assert not int8.quantize_int8(x)[0].is_inference()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_linear_does_not_depend_on_the_batch(dtype):
+    """A token's outputs are the same to the bit alone, among few and among many, whatever kernel takes the product."""
+    n, k = 2600, 272
+    x, w = _int8(2500, k, seed=1).cuda(), _int8(n, k, seed=2).cuda()
+    xs, ws = torch.rand(2500).cuda() * 0.02, torch.rand(n).cuda() * 1e-3
+    b, r = torch.randn(n).to(dtype).cuda(), torch.randn(2500, n).to(dtype).cuda()
+    for bias, residual in ((None, None), (b, None), (None, r), (b, r)):
+        full = int8.linear_int8(x, xs, w, ws, bias=bias, residual=residual, dtype=dtype)
+        for m in (1, 7, 20, 40, 100, 300, 700, 1500):
+            some = int8.linear_int8(x[:m], xs[:m], w, ws, bias=bias, residual=None if residual is None else residual[:m], dtype=dtype)
+            assert torch.equal(some, full[:m]), m
+        for cut in (1, 4):  # rows of outputs at other addresses
+            some = int8.linear_int8(x, xs, w[cut:], ws[cut:], bias=None if bias is None else bias[cut:].clone(),
+                                    residual=None if residual is None else residual[:, cut:], dtype=dtype)
+            assert torch.equal(some, full[:, cut:]), cut
+        some = int8.linear_int8(x[:9, 1:], xs[:9], w[:, 1:], ws, bias=bias, dtype=dtype)  # at odd addresses
+        many = int8.linear_int8(x[:, 1:], xs, w[:, 1:], ws, bias=bias, dtype=dtype)
+        assert torch.equal(some, many[:9])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_dequantize_rounds_the_fp32_product(dtype):
+    """Also where the product, in fp32, falls half-way between two values of the result's type: scales of few bits."""
+    q = torch.arange(-128, 128, dtype=torch.int16).to(torch.int8).repeat(20000, 1)
+    g = torch.Generator().manual_seed(3)
+    scale = torch.rand(20000, generator=g) + 0.01
+    scale[::2] = ((scale[::2] * 4096).round() + 0.5) / 4096 * (1 + 2.0 ** -23 * torch.randint(-1, 2, (10000,), generator=g))
+    for width in (256, 255, 7):
+        got = int8.dequantize_int8(q[:, :width].cuda(), scale.cuda(), dtype=dtype)
+        assert torch.equal(got.cpu(), (q[:, :width].float() * scale[:, None]).to(dtype))

@@ -113,7 +113,7 @@ def hip_sources():
 def build_hip(force=False):
     out = LIBDIR / "libtca_hip.so"
     srcs = hip_sources()
-    hdrs = list((CSRC / "hip").glob("*.h")) + list((CSRC / "hip").glob("*.hpp"))
+    hdrs = list((CSRC / "hip").glob("*.h")) + list((CSRC / "hip").glob("*.hpp")) + [Path(__file__)]  # the flags
     if not srcs:
         return None
     if force or _stale(out, srcs + hdrs):
