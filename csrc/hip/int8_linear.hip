@@ -857,11 +857,11 @@ float Estimate(const Way& w, long long m, long long n, long long k) {
 
 // Tiles at least half of whose rows would be empty are left out: few rows are bound by memory, where estimates meet.
 template <int kCount>
-int Fastest(const Way (&ways)[kCount], long long m, long long n, long long k, float* time = nullptr) {
+int Fastest(const Way (&ways)[kCount], long long m, long long n, long long k, float* time = nullptr, int most_columns = 256) {
   int best = -1;
   float least = 0.f;
   for (int i = 0; i < kCount; ++i) {
-    if (ways[i].rows > 16 && ways[i].rows >= 2 * m) continue;
+    if ((ways[i].rows > 16 && ways[i].rows >= 2 * m) || ways[i].columns > most_columns) continue;
     const float t = Estimate(ways[i], m, n, k);
     if (best < 0 || t < least) {
       best = i;
@@ -880,14 +880,20 @@ constexpr Way kAligned[] = {{256, 256, 1, 1, 1.16f, 6.96f, 0.18f, 0.80f, 0.86f},
                             {16, 32, 2, 6, 0.23f, 0.90f, 0.16f, 0.37f, 0.50f},   {16, 16, 8, 2, 0.30f, 0.90f, 0.34f, 0.69f, 0.48f},
                             {16, 16, 4, 5, 0.20f, 0.76f, 0.18f, 0.40f, 0.62f},   {16, 16, 2, 10, 0.20f, 0.73f, 0.10f, 0.24f, 0.60f}};
 
-// A large weight for up to eight tokens is bound by memory alone, and what differs is how the rows that are asked for at a
-// time fall on its channels, which the estimates do not know: narrow tiles of 16 rows do best where rows are a power of two
-// apart (1 x 16384 x 8192: 22.9 us, where 32 rows take 29.1) and as well as others elsewhere.
+// Few tokens are bound by memory, and what differs is how the rows that are asked for at a time fall on its channels, which
+// the estimates do not know: tiles of 16 weight rows do best where rows are multiples of 8 KB apart (16 x 6144 x 8192: 10.8
+// us, where 32 rows take 13.9), and for a large weight and up to eight tokens one of them does as well as any (1 x 16384 x
+// 8192: 22.9 us against 29.1 with 32 rows).
 constexpr long long kStreams = 64ll << 20;
+
+int AlignedWay(const LinearArgs& a) {
+  if (a.m <= 8 && a.n * a.k >= kStreams) return 12;
+  return Fastest(kAligned, a.m, a.n, a.k, nullptr, a.m <= 16 && a.w_stride % 8192 == 0 ? 16 : 256);
+}
 
 template <typename T>
 int LaunchAligned(const LinearArgs& a, hipStream_t st) {
-  switch (a.m <= 8 && a.n * a.k >= kStreams ? 12 : Fastest(kAligned, a.m, a.n, a.k)) {
+  switch (AlignedWay(a)) {
     case 0: return LaunchTile<T, 256, 256, 2, 2, 2, 1>(a, st);
     case 1: return LaunchTile<T, 256, 128, 2, 2, 3, 1>(a, st);
     case 2: return LaunchTile<T, 128, 128, 2, 2, 2, 2>(a, st);
