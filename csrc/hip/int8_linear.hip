@@ -14,7 +14,8 @@
 // SplitDmaKernel  few tokens or small outputs: the waves of a block share the k axis of one small output tile, every wave
 //              multiplies its own k steps of 128 from a ring of its own in LDS, filled by DMA; the sums meet in LDS.  Bound
 //              by memory: 16 x 32768 x 4096 in 25 to 28 us (4.8 to 5.4 TB/s), 1 x 4096 x 4096 in 4.5 us on the GPU.
-// SplitAnyKernel  the same for rows that do not start at multiples of 16 bytes, through registers.
+// SplitAnyKernel, TileAnyKernel  the same, and tiles of 64 x 64, for rows that do not start at multiples of 16 bytes, through
+//              registers.
 // TileKernel   large products: tiles of 64 x 64 to 256 x 256 outputs per block of four waves, operands through LDS stages
 //              filled by DMA.  8192 x 8192 x 8192 to bf16: 371 to 395 us on two cards (2.8 to 3.0 POP/s), 382 to 411 with a
 //              residual.  What bounds it is the card's power: on zeros, where nothing toggles, the same call took 296 us (312
@@ -729,6 +730,96 @@ __global__ __launch_bounds__(64 * kWM * kWN, kBlocks) void TileKernel(LinearArgs
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // nothing may arrive in this LDS after the block has left it
 }
 
+// Tiles for rows at any address, which the DMA does not take: a stage's pieces come to registers along the rows, as the
+// DMA's lanes go, while the two stages before it are multiplied, and are written to the other half of LDS behind them.  Four
+// waves.  Bound by those loads: of 16 bytes at odd addresses a CU takes in 14 to 17 bytes per cycle.  Between copying and
+// the split kernels it has its place: 672 x 1308 x 133 5.1 us (copied 7.9, split 7.1), 200 x 4096 x 4095 22.6 (24.0, 26.1).
+template <typename T, int BM, int BN, int kWM, int kWN, int kBlocks>
+__global__ __launch_bounds__(256, kBlocks) void TileAnyKernel(LinearArgs a, Tiles tiles) {
+  static_assert(kWM * kWN == 4, "four waves");
+  constexpr int kMT = BM / (16 * kWM), kNT = BN / (16 * kWN);
+  constexpr int kXPieces = BM / 32, kPieces = (BM + BN) / 32;
+  constexpr int kStageBytes = (BM + BN) * kTileK;
+  extern __shared__ __attribute__((aligned(16))) int8_t lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / kWN, wn = wave % kWN;
+  TileCursor tile;
+  tile.at = blockIdx.x >> 3;
+  tile.Place<BM, BN>(a, tiles);
+  if (tile.rows == 0) return;
+  const int8_t* const x_rows = a.x + tile.m0 * a.x_stride;
+  const int8_t* const w_rows = a.w + tile.n0 * a.w_stride;
+  const int chunk = (lane & 7) ^ (lane >> 4) ^ ((wave & 1) * 4);  // the places in LDS as in TileKernel
+  unsigned row[kPieces];  // offsets; rows past the end read the last one, their results are not stored
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    if (i < kXPieces) row[i] = min((i * 4 + wave) * 8 + (lane >> 3), tile.rows - 1) * static_cast<unsigned>(a.x_stride);
+    else row[i] = min(((i - kXPieces) * 4 + wave) * 8 + (lane >> 3), tile.columns - 1) * static_cast<unsigned>(a.w_stride);
+  }
+  const int stages = (a.k + kTileK - 1) / kTileK;
+  int4v piece[2][kPieces];  // of two stages, on their way
+  auto load = [&](int s, auto set) {
+    int4v (&to)[kPieces] = piece[decltype(set)::value];
+    const int k = s * kTileK + chunk * 16;
+    if (s * kTileK + kTileK <= a.k) {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) __builtin_memcpy(&to[i], (i < kXPieces ? x_rows : w_rows) + (row[i] + k), 16);
+    } else if (s < stages) {  // the rows end in this stage
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) to[i] = RequestPiece((i < kXPieces ? x_rows : w_rows) + row[i], k, a.k);
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i) to[i] = PieceOf(to[i], k, a.k);
+    }
+  };
+  auto store = [&](int at, auto set) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      *reinterpret_cast<int4v*>(lds + at + (i * 4 + wave) * 1024 + lane * 16) = piece[decltype(set)::value][i];
+  };
+  const int frag = (lane & 15) * kTileK + ((lane >> 4) ^ ((lane >> 1) & 7)) * 16;
+  const int x_frag = wm * (BM / kWM) * kTileK + frag;
+  const int w_frag = (BM + wn * (BN / kWN)) * kTileK + frag;
+  int4v acc[kMT][kNT];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) acc[i][j] = int4v{0, 0, 0, 0};
+  constexpr std::integral_constant<int, 0> kZero{};
+  constexpr std::integral_constant<int, 1> kOne{};
+  // stage s from its half of LDS, whose pieces were of set `mine`: those of two stages on are requested into it, and the
+  // other half, which every wave has read before the barrier behind the last stage, takes the next stage's
+  auto stage = [&](int s, int at, auto mine, auto other) {
+    load(s + 2, mine);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int4v x[kMT], w[kNT];
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) w[j] = *reinterpret_cast<const int4v*>(lds + ((at + w_frag) ^ (h * 64)) + j * 16 * kTileK);
+#pragma unroll
+      for (int i = 0; i < kMT; ++i) x[i] = *reinterpret_cast<const int4v*>(lds + ((at + x_frag) ^ (h * 64)) + i * 16 * kTileK);
+#pragma unroll
+      for (int i = 0; i < kMT; ++i)
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], x[i], acc[i][j], 0, 0, 0);
+    }
+    if (s + 1 < stages) store(kStageBytes - at, other);
+    __syncthreads();
+  };
+  load(0, kZero);
+  load(1, kOne);
+  store(0, kZero);
+  __syncthreads();
+  for (int s = 0; s < stages; s += 2) {
+    stage(s, 0, kZero, kOne);
+    if (s + 1 < stages) stage(s + 1, kStageBytes, kOne, kZero);
+  }
+  int8_t* const mine = lds + wave * (kNT * 1024);
+  const int m = wm * (BM / kWM), n = wn * (BN / kWN);
+  if (!a.vector_rows) FinishWave<T, kAny, true>(a, tile, m, n, mine, acc);
+  else FinishWave<T, kPieces, true>(a, tile, m, n, mine, acc);
+}
+
 // Rows that do not start at multiples of 16 bytes are copied to rows that do, zeros behind them: the DMA moves whole
 // 16-byte pieces.  x's rows come first, w's behind them.  A thread has kPadPieces pieces on their way at a time.
 constexpr int kPadPieces = 4;
@@ -819,6 +910,20 @@ int LaunchTile(const LinearArgs& a, hipStream_t stream) {
   return Status();
 }
 
+constexpr long long kMostTiles = 1ll << 23;  // a grid of fewer than 2^32 threads
+
+template <typename T, int BM, int BN, int kWM, int kWN, int kBlocks>
+int LaunchTileAny(const LinearArgs& a, hipStream_t stream) {
+  const long long tiles_m = (a.m + BM - 1) / BM, tiles_n = (a.n + BN - 1) / BN;
+  if (tiles_m * tiles_n > kMostTiles) return -3;
+  const Tiles tiles{static_cast<unsigned>(tiles_m), static_cast<unsigned>(tiles_n), static_cast<unsigned>((tiles_m * tiles_n + 7) / 8)};
+  constexpr int kLds = 2 * (BM + BN) * kTileK;
+  static_assert(kLds >= 16 * BN * kWM * 4 && kBlocks * kLds <= 160 * 1024, "a CU's LDS");
+  if (const int rc = AllowLds<&TileAnyKernel<T, BM, BN, kWM, kWN, kBlocks>>(kLds)) return rc;
+  hipLaunchKernelGGL((TileAnyKernel<T, BM, BN, kWM, kWN, kBlocks>), dim3(8 * tiles.run), dim3(256), kLds, stream, a, tiles);
+  return Status();
+}
+
 bool Aligned(const void* x, const void* w, long long x_stride, long long w_stride, long long k) {
   return ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w) | x_stride | w_stride | k) & 15) == 0;
 }
@@ -857,10 +962,11 @@ float Estimate(const Way& w, long long m, long long n, long long k) {
 
 // Tiles at least half of whose rows would be empty are left out: few rows are bound by memory, where estimates meet.
 template <int kCount>
-int Fastest(const Way (&ways)[kCount], long long m, long long n, long long k, float* time = nullptr, int most_columns = 256) {
+int Fastest(const Way (&ways)[kCount], long long m, long long n, long long k, float* time = nullptr, int most_columns = 256,
+            int count = kCount) {
   int best = -1;
   float least = 0.f;
-  for (int i = 0; i < kCount; ++i) {
+  for (int i = 0; i < count; ++i) {
     if ((ways[i].rows > 16 && ways[i].rows >= 2 * m) || ways[i].columns > most_columns) continue;
     const float t = Estimate(ways[i], m, n, k);
     if (best < 0 || t < least) {
@@ -913,26 +1019,35 @@ int LaunchAligned(const LinearArgs& a, hipStream_t st) {
 
 constexpr Way kUnaligned[] = {{32, 64, 4, 3, 1.27f, 3.57f, 1.22f, 1.92f, 0.25f}, {32, 32, 8, 2, 1.71f, 1.25f, 1.50f, 0.69f, 0.38f},
                               {32, 32, 4, 4, 0.82f, 2.12f, 0.79f, 0.55f, 0.25f}, {16, 32, 4, 4, 0.60f, 1.58f, 0.59f, 0.40f, 0.33f},
-                              {16, 16, 16, 1, 1.57f, 0.31f, 0.30f, 0.80f, 1.46f}, {16, 16, 4, 4, 0.45f, 1.10f, 0.41f, 0.11f, 0.46f}};
+                              {16, 16, 16, 1, 1.57f, 0.31f, 0.30f, 0.80f, 1.46f}, {16, 16, 4, 4, 0.45f, 1.10f, 0.41f, 0.11f, 0.46f},
+                              {64, 64, 1, 4, 0.58f, 1.66f, 0.42f, 0.75f, 0.24f}};
+
+bool FarApart(const LinearArgs& a) {
+  return a.x_stride > kMostStride || a.w_stride > kMostStride || a.y_stride > kMostStride || a.residual_stride > kMostStride;
+}
 
 int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
-  switch (Fastest(kUnaligned, a.m, a.n, a.k)) {
+  const bool tiles = !FarApart(a) && ((a.m + 63) / 64) * ((a.n + 63) / 64) <= kMostTiles;
+  switch (Fastest(kUnaligned, a.m, a.n, a.k, nullptr, 256, tiles ? 7 : 6)) {
     case 0: return LaunchSplitAny<2, 4, 4>(a, st);
     case 1: return LaunchSplitAny<2, 2, 8>(a, st);
     case 2: return LaunchSplitAny<2, 2, 4>(a, st);
     case 3: return LaunchSplitAny<1, 2, 4>(a, st);
     case 4: return LaunchSplitAny<1, 1, 16>(a, st);
-    default: return LaunchSplitAny<1, 1, 4>(a, st);
+    case 5: return LaunchSplitAny<1, 1, 4>(a, st);
+    default:
+      if (a.dtype == tca::kF32) return LaunchTileAny<float, 64, 64, 2, 2, 4>(a, st);
+      return a.dtype == tca::kF16 ? LaunchTileAny<_Float16, 64, 64, 2, 2, 4>(a, st) : LaunchTileAny<Bf16, 64, 64, 2, 2, 4>(a, st);
   }
 }
 
 // Copying the operands to aligned rows lets the DMA and the large tiles in; it costs a launch and the operands' bytes twice
-// (3.2 us and 0.43 us per MB).  1756 x 1856 x 4199: 29 us copied, 88 as they are; 125 x 5248 x 2315: 19.2 and 16.4.
+// (3.5 us and 0.4 us per MB).  1756 x 1856 x 4199: 29 us copied, 88 as they are; 125 x 5248 x 2315: 19.2 and 16.4.
 bool Pads(long long m, long long n, long long k) {
   float aligned, unaligned;
   Fastest(kAligned, m, n, k, &aligned);
   Fastest(kUnaligned, m, n, k, &unaligned);
-  return aligned + 3.2f + 4.3e-7f * static_cast<float>(m + n) * static_cast<float>(k) < unaligned;
+  return aligned + 3.5f + 4.0e-7f * static_cast<float>(m + n) * static_cast<float>(k) < unaligned;
 }
 
 int Launch(LinearArgs a, void* workspace, hipStream_t st) {
@@ -950,8 +1065,7 @@ int Launch(LinearArgs a, void* workspace, hipStream_t st) {
     a.x_stride = a.w_stride = row;
     a.k = pieces * 16;
   }
-  if (a.x_stride > kMostStride || a.w_stride > kMostStride || a.y_stride > kMostStride || a.residual_stride > kMostStride)
-    return LaunchUnaligned(a, st);
+  if (FarApart(a)) return LaunchUnaligned(a, st);
   if (a.dtype == tca::kF32) return LaunchAligned<float>(a, st);
   return a.dtype == tca::kF16 ? LaunchAligned<_Float16>(a, st) : LaunchAligned<Bf16>(a, st);
 }

@@ -757,3 +757,15 @@ def test_dequantize_rounds_the_fp32_product(dtype):
     for width in (256, 255, 7):
         got = int8.dequantize_int8(q[:, :width].cuda(), scale.cuda(), dtype=dtype)
         assert torch.equal(got.cpu(), (q[:, :width].float() * scale[:, None]).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(672, 1308, 133), (120, 4160, 319), (1393, 1408, 493), (65, 700, 5), (70, 3000, 17), (100, 5000, 256),
+                                   (330, 1000, 129)])
+def test_linear_in_tiles_at_any_address(m, n, k, dtype):
+    xb, wb = _int8(m, k + 24, seed=1, low=-128).cuda(), _int8(n, k + 40, seed=2, low=-128).cuda()
+    for x_at, w_at in ((0, 0), (1, 2), (7, 13), (16, 3)):
+        x, w = xb[:, x_at:x_at + k], wb[:, w_at:w_at + k]
+        for cut in (0, 3):
+            _linear_case(m - cut, n - cut, k, dtype, bias=True, residual=cut == 0, x=x[cut:].contiguous(), w=w[cut:])
+            _linear_case(m - cut, n - cut, k, dtype, x=x[cut:], w=w[cut:])
