@@ -148,7 +148,7 @@ struct RowArgs {
   long long x_stride, residual_stride, q_stride, sum_stride;
   int width;
   int weight_f32;  // the norm's weight: fp32, or the type of x
-  double eps;
+  double eps, inverse_width;
 };
 
 // g / (1 + exp(-g)), within 7 half steps of fp32 (2^-24).  With z = exp(-|g|) <= 1 it is g / (1 + z) or g z / (1 + z), in
@@ -242,10 +242,9 @@ __device__ __forceinline__ uint64_t Levels(const float (&p)[kVec], float top, fl
   float worst = 0.f;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
-    const float t = p[i] * inverse;
-    const float shifted = t + kMagic;
+    const float shifted = fmaf(p[i], inverse, kMagic);
     level[i] = __float_as_uint(shifted);
-    worst = fmaxf(worst, fabsf(t - (shifted - kMagic)));
+    worst = fmaxf(worst, fabsf(fmaf(p[i], inverse, kMagic - shifted)));
   }
   // below 2^-100 the inverse overflows or p loses bits: all of the row in 64 bits
   if (worst > 0.49996f || top < 0x1p-100f) {
@@ -334,8 +333,16 @@ __device__ __forceinline__ void StoreScale(const RowArgs& a, long long row, unsi
   if (top >= kInfBits) {
     a.scale[row] = __uint_as_float(0x7fc00000u);
   } else if constexpr (kMode == kNorm || kMode == kNormResidual) {
-    const double factor = 1.0 / sqrt(squares / a.width + a.eps);
-    a.scale[row] = static_cast<float>(static_cast<double>(__uint_as_float(top)) * factor / 127.0);
+    const double mean = fma(squares, a.inverse_width, a.eps);
+    double factor = 1.0;
+    if (mean > 0x1p-1000) {  // the unit's 24 bits and a step of third order
+      factor = __builtin_amdgcn_rsq(mean);
+      const double off = fma(-mean * factor, factor, 1.0);
+      factor = fma(factor * off, fma(0.375, off, 0.5), factor);
+    } else {
+      factor = 1.0 / sqrt(mean);
+    }
+    a.scale[row] = static_cast<float>(static_cast<double>(__uint_as_float(top)) * factor * (1.0 / 127.0));
   } else {
     // next to the largest fp32 value 127 s can round to infinity: there s is the next smaller number
     const float s = __uint_as_float(top) / 127.f;
@@ -580,6 +587,7 @@ int tca_int8_rms_norm_launch(const void* x, const void* residual, const void* we
   a.sum_stride = sum_stride;
   a.weight_f32 = weight_f32;
   a.eps = eps;
+  a.inverse_width = 1.0 / static_cast<double>(width);
   return Rows(residual ? kNormResidual : kNorm, dtype, a, stream);
 }
 
