@@ -1,6 +1,6 @@
 // The 8-bit operators' calls on torch tensors without the interpreter in between: checks, result allocation and launch of
 // the plain case - contiguous CUDA tensors of the right types and shapes on the current device, new results.  For
-// everything else (strided operands, destinations, other devices, gradients, wrong arguments, a failed launch) the
+// everything else (strided operands, destinations, other devices, gradients, traces, wrong arguments, a failed launch) the
 // functions return None and the Python operators go their general way, which also words the errors.  A call costs 3.3 to
 // 4.3 us this way (two hosts), 2.8 of them the launch itself, instead of 8 to 13.
 //
@@ -8,7 +8,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
@@ -41,16 +43,18 @@ at::ScalarType Type(long code) { return code == 0 ? at::kFloat : code == 1 ? at:
 
 constexpr long long kMostWidth = 1ll << 29, kMostK = 131071;
 
-// A plain operand: a contiguous tensor on the current CUDA device that needs no gradient.  `device` is set by the first
-// operand (-1 before it): without a GPU there is no current device to ask for.
+// A plain operand: a contiguous tensor on the current CUDA device that needs no gradient and has no tangent, in a call that
+// nothing traces.  `device` is set by the first operand (-1 before it): without a GPU there is no current device to ask for.
 struct Operand {
   const at::Tensor* t = nullptr;
   bool Take(PyObject* o, int& device) {
     if (!THPVariable_CheckExact(o)) return false;
     t = &THPVariable_Unpack(o);
-    if (!t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous() || t->requires_grad() || t->is_conj() || t->is_neg())
+    if (!t->is_cuda() || t->layout() != at::kStrided || !t->is_contiguous() || t->requires_grad() || t->is_conj() || t->is_neg() ||
+        t->_fw_grad(0).defined())
       return false;
     if (device < 0) {
+      if (at::tracer::impl::is_dispatch_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
       device = t->device().index();
       return c10::hip::current_device() == device;
     }

@@ -769,3 +769,39 @@ def test_linear_in_tiles_at_any_address(m, n, k, dtype):
         for cut in (0, 3):
             _linear_case(m - cut, n - cut, k, dtype, bias=True, residual=cut == 0, x=x[cut:].contiguous(), w=w[cut:])
             _linear_case(m - cut, n - cut, k, dtype, x=x[cut:], w=w[cut:])
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_tangents_and_traces_on_the_gpu():
+    """Refused on the extension's way too, and plain calls again once the level or the trace has ended."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from triton_client_amd import _native
+
+    ops = _native.torch_ops()
+    x = _values(3, 32, torch.float16).cuda()
+    q, s = int8.quantize_int8(x)
+
+    def calls(x, s):
+        return (lambda: int8.quantize_int8(x), lambda: int8.silu_mul_int8(x), lambda: int8.dequantize_int8(q, s),
+                lambda: int8.rms_norm_int8(x, x[0], residual=x), lambda: int8.linear_int8(q, s, q, s))
+
+    with forward_ad.dual_level():
+        xd, sd = forward_ad.make_dual(x, x), forward_ad.make_dual(s, s)
+        assert ops.quantize(xd, False) is None and ops.dequantize(q, sd, 1) is None
+        for call in calls(xd, sd):
+            with pytest.raises(ValueError, match="no derivative"):
+                call()
+        assert ops.quantize(x, False) is not None
+
+    def traced(x):
+        assert ops.quantize(x, False) is None
+        for call in calls(x, s):
+            with pytest.raises(ValueError, match="traced"):
+                call()
+        return x + 1
+
+    torch.jit.trace(traced, (x,), check_trace=False)
+    make_fx(traced)(x)
+    assert torch.equal(ops.quantize(x, False)[0], q)

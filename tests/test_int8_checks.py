@@ -146,3 +146,50 @@ def test_without_the_extension(monkeypatch):
         int8.quantize_int8(_x(2, 8))
     with pytest.raises(ValueError, match="CUDA"):  # and no second warning
         int8.quantize_int8(_x(2, 8))
+
+
+def _every_call(x):
+    """Each operator on ``x [2, 8]`` in one of its places."""
+    q, s = _x(2, 8, dtype=torch.int8), torch.ones(2)
+    return (lambda: int8.quantize_int8(x), lambda: int8.silu_mul_int8(x), lambda: int8.rms_norm_int8(x, torch.ones(8)),
+            lambda: int8.rms_norm_int8(torch.ones(2, 8), x[0]), lambda: int8.dequantize_int8(q, x[:, 0]),
+            lambda: int8.rms_norm_int8(torch.ones(2, 8), torch.ones(8), residual=x),
+            lambda: int8.dequantize_int8(q, s, out=x), lambda: _linear(x_scale=x[0, :3]),
+            lambda: _linear(dtype=torch.float32, bias=x[0, :4]))
+
+
+def test_tangents_are_refused():
+    """A dual tensor requires no gradient, and its tangent would be lost; also where no gradient is recorded, which does
+    not end the forward mode."""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.ones(2, 8), torch.ones(2, 8))
+        for call in _every_call(x):
+            with pytest.raises(ValueError, match="no derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(ValueError, match="no derivative"):
+                call()
+        with pytest.raises(ValueError, match="CUDA"):
+            int8.quantize_int8(forward_ad.unpack_dual(x).primal)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traces_are_refused():
+    """A trace would hold the results as constants."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    seen = []
+
+    def f(x):
+        for call in _every_call(x):
+            with pytest.raises(ValueError, match="traced"):
+                call()
+            seen.append(1)
+        return x + 1
+
+    torch.jit.trace(f, (torch.ones(2, 8),), check_trace=False)
+    make_fx(f)(torch.ones(2, 8))
+    assert len(seen) == 2 * len(_every_call(torch.ones(2, 8)))
+    with pytest.raises(ValueError, match="CUDA"):
+        int8.quantize_int8(torch.ones(2, 8))

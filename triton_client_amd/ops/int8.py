@@ -20,7 +20,8 @@ activations crossing memory in 8 bits between the products::
 Rows are everything but the last axis.  Inputs are torch CUDA tensors of fp16, bf16 or fp32 (integers: int8); rows may
 lie apart (a 2-D view with a row stride), other layouts are copied first.  Work is enqueued on the current torch stream
 of the tensors' device and nothing waits for it; results may be captured into graphs.  The integers have no gradient:
-operands that require one are refused while gradients are recorded.
+operands that require one are refused while gradients are recorded, those with a forward-mode tangent always, and so
+are calls inside ``torch.jit.trace`` or ``make_fx``, which would record the results as constants.
 
 A row with a value that is not finite gets integers of 0 and a scale of NaN, so that whatever is computed from it is NaN
 instead of a number.  The reference has no model code (its models run in the server it talks to, e.g.
@@ -30,9 +31,11 @@ instead of a number.  The reference has no model code (its models run in the ser
 from __future__ import annotations
 
 import subprocess
+import sys
 import warnings
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 from ._device import check, lib
@@ -75,20 +78,32 @@ def _output_code(dtype):
 
 
 def _check_operands(first, others):
-    """Index of the operands' common CUDA device; no operand may require a gradient while gradients are recorded, nor
-    stand for other values than those in memory."""
+    """Index of the operands' common CUDA device; no operand may require a gradient while gradients are recorded, carry a
+    tangent, or stand for other values than those in memory, and no trace may be under way."""
     device = first.get_device()
+    duals = getattr(forward_ad, "_current_level", 0) >= 0  # tangents live inside a level
     for t in (first, *others):
         if t is not None:
             if t.requires_grad:
                 _refuse_gradient()
+            if duals and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("8-bit operators have no derivative: take the primal of forward_ad.unpack_dual()")
             if t.is_neg():
                 raise ValueError("an operand's negation is pending: call its resolve_neg()")
             if t.get_device() != device:
                 raise ValueError("the operands must be on one device")
+    # what launches a kernel by itself would enter a trace as a constant
+    if torch.jit.is_tracing() or _proxy_mode():
+        raise ValueError("8-bit operators cannot be traced: call them outside of the traced function")
     if device < 0:
         raise ValueError("the operands must be CUDA tensors")
     return device
+
+
+def _proxy_mode():
+    """Whether ``make_fx`` records the operations of this thread."""
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")  # there if one does
+    return proxies is not None and proxies.get_proxy_mode() is not None
 
 
 def _refuse_gradient():
