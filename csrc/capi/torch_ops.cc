@@ -17,23 +17,22 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <iterator>
+#include <limits>
+#include <type_traits>
+
+#include "kernels.h"
+
 namespace py = pybind11;
 
 namespace {
 
-using QuantizeFn = int (*)(const void*, void*, void*, int, int, long long, long long, long long, long long, void*);
-using NormFn = int (*)(const void*, const void*, const void*, void*, void*, void*, int, int, double, long long, long long,
-                       long long, long long, long long, long long, void*);
-using DequantizeFn = int (*)(const void*, const void*, void*, int, long long, long long, long long, long long, void*);
-using LinearFn = int (*)(const void*, const void*, const void*, const void*, const void*, const void*, void*, int, long long,
-                         long long, long long, long long, long long, long long, long long, void*, void*);
-using WorkspaceFn = long long (*)(const void*, const void*, long long, long long, long long, long long, long long);
-
-QuantizeFn g_quantize;
-NormFn g_norm;
-DequantizeFn g_dequantize;
-LinearFn g_linear;
-WorkspaceFn g_workspace;
+// called through their declarations: a launcher whose arguments change does not compile here until its call does
+decltype(&tca_int8_quantize_launch) g_quantize;
+decltype(&tca_int8_rms_norm_launch) g_norm;
+decltype(&tca_int8_dequantize_launch) g_dequantize;
+decltype(&tca_int8_linear_launch) g_linear;
+decltype(&tca_int8_linear_workspace_bytes) g_workspace;
 
 // element type codes of the kernels, -1: another type
 int Code(at::ScalarType t) {
@@ -209,15 +208,33 @@ PyObject* Linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// addresses of the launchers: quantize, rms_norm, dequantize, linear, linear_workspace_bytes
-PyObject* Use(PyObject*, PyObject* args) {
-  unsigned long long p[5];
-  if (!PyArg_ParseTuple(args, "KKKKK", &p[0], &p[1], &p[2], &p[3], &p[4])) return nullptr;
-  g_quantize = reinterpret_cast<QuantizeFn>(p[0]);
-  g_norm = reinterpret_cast<NormFn>(p[1]);
-  g_dequantize = reinterpret_cast<DequantizeFn>(p[2]);
-  g_linear = reinterpret_cast<LinearFn>(p[3]);
-  g_workspace = reinterpret_cast<WorkspaceFn>(p[4]);
+// the launchers that are called here, as `launchers` names them, and where `use` puts their addresses
+template <auto& kFunction>
+void Set(unsigned long long address) {
+  kFunction = reinterpret_cast<std::remove_reference_t<decltype(kFunction)>>(address);
+}
+struct Launcher {
+  const char* name;
+  void (*set)(unsigned long long);
+};
+constexpr Launcher kLaunchers[] = {{"tca_int8_quantize_launch", Set<g_quantize>},
+                                   {"tca_int8_rms_norm_launch", Set<g_norm>},
+                                   {"tca_int8_dequantize_launch", Set<g_dequantize>},
+                                   {"tca_int8_linear_launch", Set<g_linear>},
+                                   {"tca_int8_linear_workspace_bytes", Set<g_workspace>}};
+
+// the launchers' addresses, in that order
+PyObject* Use(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != static_cast<Py_ssize_t>(std::size(kLaunchers))) {
+    PyErr_SetString(PyExc_TypeError, "an address for each of the launchers");
+    return nullptr;
+  }
+  unsigned long long addresses[std::size(kLaunchers)];
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    addresses[i] = PyLong_AsUnsignedLongLong(args[i]);
+    if (PyErr_Occurred()) return nullptr;
+  }
+  for (Py_ssize_t i = 0; i < n; ++i) kLaunchers[i].set(addresses[i]);
   Py_RETURN_NONE;
 }
 
@@ -225,7 +242,7 @@ PyCFunction Fast(PyObject* (*f)(PyObject*, PyObject* const*, Py_ssize_t)) {
   return reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f));
 }
 
-PyMethodDef kMethods[] = {{"use", Use, METH_VARARGS, nullptr},
+PyMethodDef kMethods[] = {{"use", Fast(Use), METH_FASTCALL, nullptr},
                           {"quantize", Fast(Quantize), METH_FASTCALL, nullptr},
                           {"rms_norm", Fast(Norm), METH_FASTCALL, nullptr},
                           {"dequantize", Fast(Dequantize), METH_FASTCALL, nullptr},
@@ -236,4 +253,16 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_tca_torch", nullptr, -1, kMethod
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tca_torch() { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__tca_torch() {
+  PyObject* module = PyModule_Create(&kModule);
+  PyObject* names = PyTuple_New(std::size(kLaunchers));
+  for (size_t i = 0; names && i < std::size(kLaunchers); ++i) {
+    PyObject* name = PyUnicode_FromString(kLaunchers[i].name);
+    if (!name) Py_CLEAR(names);
+    else PyTuple_SET_ITEM(names, i, name);
+  }
+  if (module && names && PyModule_AddObject(module, "launchers", names) == 0) return module;  // names belongs to it now
+  Py_XDECREF(names);
+  Py_XDECREF(module);
+  return nullptr;
+}

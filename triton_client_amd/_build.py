@@ -96,12 +96,12 @@ def build_torch(force=False):
     home = Path(list(spec.submodule_search_locations)[0])
     out = LIBDIR / f"_tca_torch{sysconfig.get_config_var('EXT_SUFFIX')}"
     src = CSRC / "capi" / "torch_ops.cc"
-    if force or _stale(out, [src, home / "version.py"]):
+    if force or _stale(out, [src, CSRC / "hip" / "kernels.h", home / "version.py"]):
         LIBDIR.mkdir(exist_ok=True)
         _compile_atomic(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
                          "-isystem", home / "include", "-isystem",
                          home / "include" / "torch" / "csrc" / "api" / "include", "-isystem", ROCM / "include",
-                         "-isystem", sysconfig.get_paths()["include"], "-o", out, src, f"-L{home / 'lib'}",
+                         "-isystem", sysconfig.get_paths()["include"], "-I", CSRC / "hip", "-o", out, src, f"-L{home / 'lib'}",
                          "-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"], out)
     return out
 

@@ -173,9 +173,7 @@ def torch_ops():
             _build.build_torch()
             from ._lib import _tca_torch
         lib = hip()
-        _tca_torch.use(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "tca_int8_quantize_launch", "tca_int8_rms_norm_launch", "tca_int8_dequantize_launch",
-            "tca_int8_linear_launch", "tca_int8_linear_workspace_bytes")))
+        _tca_torch.use(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _tca_torch.launchers))
         _torch_ops = _tca_torch
     return _torch_ops
 
