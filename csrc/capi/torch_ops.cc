@@ -4,6 +4,9 @@
 // functions return None and the Python operators go their general way, which also words the errors.  A call costs 3.3 to
 // 4.3 us this way (two hosts), 2.8 of them the launch itself, instead of 8 to 13.
 //
+// Accessors of torch's tensors are compiled in, so the module serves the torch that it was built for, which `built_for`
+// names (the build passes TCA_TORCH); the loader leaves it alone under any other.
+//
 // The launchers come as addresses: libtca_hip.so is loaded by its own loader.
 #include <Python.h>
 
@@ -261,7 +264,9 @@ PyMODINIT_FUNC PyInit__tca_torch() {
     if (!name) Py_CLEAR(names);
     else PyTuple_SET_ITEM(names, i, name);
   }
-  if (module && names && PyModule_AddObject(module, "launchers", names) == 0) return module;  // names belongs to it now
+  if (module && names && PyModule_AddStringConstant(module, "built_for", TCA_TORCH) == 0 &&
+      PyModule_AddObject(module, "launchers", names) == 0)
+    return module;  // names belongs to it now
   Py_XDECREF(names);
   Py_XDECREF(module);
   return nullptr;

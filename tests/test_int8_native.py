@@ -78,3 +78,56 @@ def test_the_extension_depends_on_the_declarations(monkeypatch):
     monkeypatch.setattr(_build, "_stale", lambda out, sources: seen.extend(sources))
     _build.build_torch()
     assert HIP / "kernels.h" in seen
+
+
+class _OtherTorch:
+    """An extension that loads, built for another torch."""
+
+    built_for = "1.0.0 0123456789"
+    launchers = ("tca_int8_quantize_launch",)
+
+    @staticmethod
+    def use(*addresses):
+        raise AssertionError("it must not be used")
+
+
+@pytest.mark.parametrize("names_it", [True, False])
+def test_an_extension_for_another_torch_is_left_alone(monkeypatch, names_it):
+    torch = pytest.importorskip("torch")
+    from triton_client_amd import _lib, _native
+    from triton_client_amd.ops import int8
+
+    if not names_it:
+        monkeypatch.delattr(_OtherTorch, "built_for")
+    monkeypatch.setattr(_native, "_torch_ops", None)
+    monkeypatch.setattr(_lib, "_tca_torch", _OtherTorch, raising=False)
+    with pytest.raises(ImportError, match="was built for torch"):
+        _native.torch_ops()
+    # the operators then go their general way
+    monkeypatch.setattr(int8, "_plain", None)
+    with pytest.warns(RuntimeWarning, match="was built for torch"), pytest.raises(ValueError, match="CUDA"):
+        int8.quantize_int8(torch.zeros(2, 8))
+
+
+def test_the_extension_is_built_again_for_another_torch(monkeypatch, tmp_path):
+    """Also where its file is newer than that torch's."""
+    torch = pytest.importorskip("torch")
+    built = []
+    monkeypatch.setattr(_build, "LIBDIR", tmp_path)
+    monkeypatch.setattr(_build, "_compile_atomic", lambda cmd, out: (built.append(cmd), out.write_bytes(b"")))
+    _build.build_torch()
+    _build.build_torch()
+    assert len(built) == 1 and f'-DTCA_TORCH="{torch.__version__} {torch.version.git_version}"' in built[0]
+    (tmp_path / "_tca_torch.torch").write_text("1.0.0 0123456789")
+    _build.build_torch()
+    assert len(built) == 2
+    (tmp_path / "_tca_torch.torch").unlink()
+    _build.build_torch()
+    assert len(built) == 3
+
+
+def test_the_built_extension_names_its_torch():
+    torch = pytest.importorskip("torch")
+    from triton_client_amd import _native
+
+    assert _native.torch_ops().built_for == f"{torch.__version__} {torch.version.git_version}"

@@ -21,6 +21,7 @@ A target is rebuilt only when one of its sources is newer than its output.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -96,13 +97,19 @@ def build_torch(force=False):
     home = Path(list(spec.submodule_search_locations)[0])
     out = LIBDIR / f"_tca_torch{sysconfig.get_config_var('EXT_SUFFIX')}"
     src = CSRC / "capi" / "torch_ops.cc"
-    if force or _stale(out, [src, CSRC / "hip" / "kernels.h", home / "version.py"]):
+    version = (home / "version.py").read_text()
+    # as _native.torch_ops() puts it together from the imported torch
+    torch = " ".join(re.search(rf"^{name} = ['\"](.*)['\"]", version, re.M).group(1) for name in ("__version__", "git_version"))
+    built_for = LIBDIR / "_tca_torch.torch"
+    if (force or _stale(out, [src, CSRC / "hip" / "kernels.h", home / "version.py"])
+            or not built_for.exists() or built_for.read_text() != torch):
         LIBDIR.mkdir(exist_ok=True)
         _compile_atomic(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
-                         "-isystem", home / "include", "-isystem",
+                         f'-DTCA_TORCH="{torch}"', "-isystem", home / "include", "-isystem",
                          home / "include" / "torch" / "csrc" / "api" / "include", "-isystem", ROCM / "include",
                          "-isystem", sysconfig.get_paths()["include"], "-I", CSRC / "hip", "-o", out, src, f"-L{home / 'lib'}",
                          "-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-ltorch", "-lc10_hip", "-lc10"], out)
+        built_for.write_text(torch)
     return out
 
 

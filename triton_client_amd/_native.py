@@ -160,10 +160,11 @@ _torch_ops = None
 
 
 def torch_ops():
-    """The ``_tca_torch`` CPython extension (built on demand), with the launchers of libtca_hip.so handed to it."""
+    """The ``_tca_torch`` CPython extension (built on demand), with the launchers of libtca_hip.so handed to it.  One that
+    was built for another torch may load and read tensors at other offsets: that is an ImportError, too."""
     global _torch_ops
     if _torch_ops is None:
-        import torch  # noqa: F401 - its libraries have to be there before the extension's symbols are bound
+        import torch  # its libraries have to be there before the extension's symbols are bound
 
         try:
             from ._lib import _tca_torch
@@ -172,6 +173,11 @@ def torch_ops():
 
             _build.build_torch()
             from ._lib import _tca_torch
+        here = f"{torch.__version__} {torch.version.git_version}"
+        built_for = getattr(_tca_torch, "built_for", "one that it does not name")
+        if built_for != here:
+            raise ImportError(f"_tca_torch was built for torch {built_for}, this is {here}: "
+                              "python -m triton_client_amd._build torch builds it again")
         lib = hip()
         _tca_torch.use(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _tca_torch.launchers))
         _torch_ops = _tca_torch
