@@ -805,3 +805,53 @@ def test_tangents_and_traces_on_the_gpu():
     torch.jit.trace(traced, (x,), check_trace=False)
     make_fx(traced)(x)
     assert torch.equal(ops.quantize(x, False)[0], q)
+
+
+def test_destinations_that_a_backward_pass_has_saved():
+    """Writing to one is found out when the gradient is taken, as after any of torch's operators in place."""
+    rows = _values(4, 32, torch.float32).cuda()
+    weight = torch.ones(32, device="cuda")
+    q, s = int8.quantize_int8(rows)
+    wq, ws = int8.quantize_int8(torch.eye(32, device="cuda"))
+    writes = [(rows, lambda t: int8.rms_norm_int8(t, weight, residual=rows, sum_out=t)),
+              (rows, lambda t: int8.rms_norm_int8(rows, weight, residual=t, sum_out=t)),
+              (rows, lambda t: int8.dequantize_int8(q, s, out=t)), (rows, lambda t: int8.dequantize_int8(q, s, out=t.view(4, 32))),
+              (rows, lambda t: int8.linear_int8(q, s, wq, ws, residual=t, out=t)), (s, lambda t: int8.quantize_int8(rows, scale=t)),
+              (s, lambda t: int8.rms_norm_int8(rows, weight, scale=t))]
+    for like, write in writes:
+        t, p = like.clone(), torch.ones_like(like, requires_grad=True)
+        y = (t * p).sum()  # saves t for p's gradient
+        version = t._version
+        write(t)
+        assert t._version == version + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    t = torch.empty(4, 32, dtype=torch.int8, device="cuda")
+    int8.quantize_int8(rows, out=t)
+    assert t._version == 1
+    # inputs and untouched destinations keep their versions; inference tensors, which have none, are written all the same
+    assert rows._version == weight._version == q._version == s._version == 0
+    empty = torch.empty(0, 32, device="cuda")
+    int8.dequantize_int8(q[:0], s[:0], out=empty)
+    assert empty._version == 0
+    with torch.inference_mode():
+        t = torch.empty(4, 32, device="cuda")
+    int8.dequantize_int8(q, s, out=t)
+    with torch.inference_mode():
+        int8.dequantize_int8(q, s, out=t)
+    assert torch.equal(t, int8.dequantize_int8(q, s, dtype=torch.float32))
+
+
+def test_destinations_in_a_graph():
+    """A capture enqueues, replays write: the version counts the call, and replays are as eager calls."""
+    rows = _values(4, 32, torch.float32).cuda()
+    q, s = int8.quantize_int8(rows)
+    t = torch.zeros(4, 32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        int8.dequantize_int8(q, s, out=t)
+    for _ in range(3):
+        t.zero_()
+        graph.replay()
+        assert torch.equal(t, int8.dequantize_int8(q, s, dtype=torch.float32))

@@ -189,6 +189,14 @@ def _launch(what, device, *args):
         check(rc, what)
 
 
+def _written(*destinations):
+    """A caller's tensors have other values now: a backward pass that has saved one of them has to find out, as it does
+    after torch's own operators.  (Inference tensors have no version, and no backward pass saves them.)"""
+    for t in destinations:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def _row_outputs(x, shape, out, scale):
     """``(q, q stride, scale)``: the destinations given, or new ones."""
     if out is None:
@@ -228,6 +236,7 @@ def _quantize(x, gated, out, scale):
     if rows:
         _launch("tca_int8_quantize_launch", device, x.data_ptr(), q.data_ptr(), s.data_ptr(), code, gated, rows,
                 shape[-1], x_stride, q_stride)
+        _written(out, scale)
     return q, s
 
 
@@ -308,6 +317,7 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_
     if rows:
         _launch("tca_int8_rms_norm_launch", device, x.data_ptr(), r_ptr, weight.data_ptr(), q.data_ptr(), s.data_ptr(),
                 sum_ptr, code, weight_f32, eps, rows, width, x_stride, r_stride, q_stride, sum_stride)
+        _written(out, scale, sum_out)
     return (q, s) if residual is None else (q, s, summed)
 
 
@@ -337,7 +347,7 @@ def dequantize_int8(q, scale, dtype=None, out=None):
     code = _output_code(dtype)
     device = _check_operands(scale, (q, out))
     q, q_stride = _rows(q)
-    scale = scale.contiguous()
+    scale, given = scale.contiguous(), out
     if out is None:
         out, out_stride = torch.empty(shape, dtype=dtype, device=q.device), shape[-1]
     else:
@@ -347,6 +357,7 @@ def dequantize_int8(q, scale, dtype=None, out=None):
     if rows:
         _launch("tca_int8_dequantize_launch", device, q.data_ptr(), scale.data_ptr(), out.data_ptr(), code, rows,
                 shape[-1], q_stride, out_stride)
+        _written(given)
     return out
 
 
@@ -387,7 +398,7 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
     x, x_stride = _rows(x)
     weight, w_stride = _rows(weight)
     x_scale, weight_scale = x_scale.contiguous(), weight_scale.contiguous()
-    r_ptr, r_stride = None, 0
+    r_ptr, r_stride, given = None, 0, out
     if residual is not None:
         residual, r_stride = _rows(residual)
         r_ptr = residual.data_ptr()
@@ -407,4 +418,5 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
         _launch("tca_int8_linear_launch", device, x_ptr, x_scale.data_ptr(), w_ptr, weight_scale.data_ptr(),
                 None if bias is None else bias.data_ptr(), r_ptr, out.data_ptr(), code, tokens, n, k, x_stride,
                 w_stride, r_stride, out_stride, None if workspace is None else workspace.data_ptr())
+        _written(given)
     return out
