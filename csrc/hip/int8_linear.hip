@@ -998,8 +998,8 @@ int AlignedWay(const LinearArgs& a) {
 }
 
 template <typename T>
-int LaunchAligned(const LinearArgs& a, hipStream_t st) {
-  switch (AlignedWay(a)) {
+int LaunchAligned(int way, const LinearArgs& a, hipStream_t st) {
+  switch (way) {
     case 0: return LaunchTile<T, 256, 256, 2, 2, 2, 1>(a, st);
     case 1: return LaunchTile<T, 256, 128, 2, 2, 3, 1>(a, st);
     case 2: return LaunchTile<T, 128, 128, 2, 2, 2, 2>(a, st);
@@ -1026,9 +1026,13 @@ bool FarApart(const LinearArgs& a) {
   return a.x_stride > kMostStride || a.w_stride > kMostStride || a.y_stride > kMostStride || a.residual_stride > kMostStride;
 }
 
-int LaunchUnaligned(const LinearArgs& a, hipStream_t st) {
+int UnalignedWay(const LinearArgs& a) {
   const bool tiles = !FarApart(a) && ((a.m + 63) / 64) * ((a.n + 63) / 64) <= kMostTiles;
-  switch (Fastest(kUnaligned, a.m, a.n, a.k, nullptr, 256, tiles ? 7 : 6)) {
+  return Fastest(kUnaligned, a.m, a.n, a.k, nullptr, 256, tiles ? 7 : 6);
+}
+
+int LaunchUnaligned(int way, const LinearArgs& a, hipStream_t st) {
+  switch (way) {
     case 0: return LaunchSplitAny<2, 4, 4>(a, st);
     case 1: return LaunchSplitAny<2, 2, 8>(a, st);
     case 2: return LaunchSplitAny<2, 2, 4>(a, st);
@@ -1050,24 +1054,45 @@ bool Pads(long long m, long long n, long long k) {
   return aligned + 3.5f + 4.0e-7f * static_cast<float>(m + n) * static_cast<float>(k) < unaligned;
 }
 
-int Launch(LinearArgs a, void* workspace, hipStream_t st) {
+// How a product is computed: the entry of kAligned or, less `any`, of kUnaligned, and whether its operands are copied first.
+struct Choice {
+  bool copied, any;
+  int way;
+};
+
+// `a` becomes what the kernel is called with: where the operands are copied, rows of the workspace.
+Choice Choose(LinearArgs& a, void* workspace) {
+  Choice c{};
   if (!Aligned(a.x, a.w, a.x_stride, a.w_stride, a.k)) {
-    if (!Pads(a.m, a.n, a.k)) return LaunchUnaligned(a, st);
+    c.copied = Pads(a.m, a.n, a.k);
+    c.any = !c.copied;
+    if (c.copied) {
+      const int row = PaddedRow(a.k);
+      a.x = static_cast<const int8_t*>(workspace);
+      a.w = workspace ? a.x + a.m * row : nullptr;
+      a.x_stride = a.w_stride = row;
+      a.k = (a.k + 15) / 16 * 16;
+    }
+  }
+  c.any = c.any || FarApart(a);
+  c.way = c.any ? UnalignedWay(a) : AlignedWay(a);
+  return c;
+}
+
+int Launch(const LinearArgs& given, void* workspace, hipStream_t st) {
+  LinearArgs a = given;
+  const Choice c = Choose(a, workspace);
+  if (c.copied) {
     if (!workspace) return -4;
-    const int row = PaddedRow(a.k);
-    const int pieces = (a.k + 15) / 16;
+    const int pieces = a.k / 16;
     const long long blocks = ((a.m + a.n) * pieces + 256 * kPadPieces - 1) / (256 * kPadPieces);
     if (blocks >= 1 << 24) return -3;
-    hipLaunchKernelGGL(PadKernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, a, static_cast<int8_t*>(workspace), pieces,
-                       row);
-    a.x = static_cast<const int8_t*>(workspace);
-    a.w = a.x + a.m * row;
-    a.x_stride = a.w_stride = row;
-    a.k = pieces * 16;
+    hipLaunchKernelGGL(PadKernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, given, static_cast<int8_t*>(workspace), pieces,
+                       static_cast<int>(a.x_stride));
   }
-  if (FarApart(a)) return LaunchUnaligned(a, st);
-  if (a.dtype == tca::kF32) return LaunchAligned<float>(a, st);
-  return a.dtype == tca::kF16 ? LaunchAligned<_Float16>(a, st) : LaunchAligned<Bf16>(a, st);
+  if (c.any) return LaunchUnaligned(c.way, a, st);
+  if (a.dtype == tca::kF32) return LaunchAligned<float>(c.way, a, st);
+  return a.dtype == tca::kF16 ? LaunchAligned<_Float16>(c.way, a, st) : LaunchAligned<Bf16>(c.way, a, st);
 }
 
 }  // namespace
@@ -1079,6 +1104,25 @@ long long tca_int8_linear_workspace_bytes(const void* x, const void* w, long lon
                                           long long w_stride) {
   if (m <= 0 || n <= 0 || k <= 0 || Aligned(x, w, x_stride, w_stride, k) || !Pads(m, n, k)) return 0;
   return (m + n) * PaddedRow(k);
+}
+
+// Which kernel takes a product of these operands: 0 to 13 the tiles for aligned rows, 16 to 22 those for rows at any address;
+// 32 more where the operands are copied to aligned rows first.  -1 for operands that a launch refuses.
+int tca_int8_linear_way(const void* x, const void* w, long long m, long long n, long long k, long long x_stride, long long w_stride,
+                        long long residual_stride, long long y_stride) {
+  if (m <= 0 || n <= 0 || k <= 0 || k > 131071) return -1;
+  LinearArgs a{};
+  a.x = static_cast<const int8_t*>(x);
+  a.w = static_cast<const int8_t*>(w);
+  a.m = m;
+  a.n = n;
+  a.k = static_cast<int>(k);
+  a.x_stride = x_stride;
+  a.w_stride = w_stride;
+  a.residual_stride = residual_stride;
+  a.y_stride = y_stride;
+  const Choice c = Choose(a, nullptr);
+  return (c.copied ? 32 : 0) + (c.any ? 16 : 0) + c.way;
 }
 
 int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, const void* w_scale, const void* bias,

@@ -134,4 +134,7 @@ int tca_int8_linear_launch(const void* x, const void* x_scale, const void* w, co
                            void* workspace, void* stream);
 long long tca_int8_linear_workspace_bytes(const void* x, const void* w, long long m, long long n, long long k, long long x_stride,
                                           long long w_stride);
+// which kernel takes such a product (see there)
+int tca_int8_linear_way(const void* x, const void* w, long long m, long long n, long long k, long long x_stride, long long w_stride,
+                        long long residual_stride, long long y_stride);
 }

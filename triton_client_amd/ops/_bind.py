@@ -159,6 +159,9 @@ def install(lib):
     lib.tca_int8_linear_workspace_bytes.restype = c_longlong
     lib.tca_int8_linear_workspace_bytes.argtypes = [c_void_p, c_void_p, c_longlong, c_longlong, c_longlong, c_longlong,
                                                     c_longlong]
+    lib.tca_int8_linear_way.restype = c_int
+    lib.tca_int8_linear_way.argtypes = [c_void_p, c_void_p, c_longlong, c_longlong, c_longlong, c_longlong, c_longlong,
+                                        c_longlong, c_longlong]
     install_rt(lib)
 
 
