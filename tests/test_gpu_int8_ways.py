@@ -4,6 +4,8 @@ Which kernel takes a product follows from estimated times, so a list of sizes sa
 names the kernel it is for (as ``tca_int8_linear_way`` numbers them: 0 to 13 tiles for aligned rows, 16 to 22 for rows at any
 address, 32 more where the operands are copied first).  That it still goes there is asserted without a GPU; the products run
 on one."""
+import threading
+
 import pytest
 import torch
 
@@ -117,3 +119,80 @@ def test_each_kernel(way, m, n, k, dtype):
         assert (rows[0] == 7).all() and (rows[-1] == 7).all() and (rows[:, n:] == 7).all()
         plain = int8.linear_int8(x, xs, w, ws, bias=bias, residual=residual, dtype=dtype)
         assert torch.equal(plain, out)
+
+
+# sizes whose operands are copied to a workspace of the call
+WITH_WORKSPACE = [(1100, 1201, 1333), (2500, 2600, 399)]
+
+
+def test_the_workspace_cases_have_one():
+    for size in WITH_WORKSPACE:
+        assert _workspace(*size) > 0, size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", WITH_WORKSPACE)
+def test_workspaces_of_two_threads(m, n, k):
+    """Calls of two threads, each on a stream of its own, their workspaces in flight at the same time."""
+    cases = []
+    for seed in range(2):
+        x, xs, w, ws, _, _ = _operands(m, n, k, torch.bfloat16, seed)
+        want = int8.linear_int8(x, xs, w, ws, dtype=torch.bfloat16)
+        ref, slack = _linear_reference(x, xs, w, ws, None, None, torch.bfloat16)
+        assert ((want.double() - ref).abs() <= slack).all()
+        cases.append((x, xs, w, ws, want))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(x, xs, w, ws, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    if not torch.equal(int8.linear_int8(x, xs, w, ws, dtype=torch.bfloat16), want):
+                        bad.append("a result differs")
+        except Exception as e:  # noqa: BLE001 - reported by the test's own thread
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=c) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", WITH_WORKSPACE)
+def test_workspaces_in_graphs(m, n, k):
+    """Captured twice; replayed with eager calls between, and on two streams at the same time."""
+    x, xs, w, ws, _, _ = _operands(m, n, k, torch.float16)
+    inputs = [torch.roll(x, shift, 0) for shift in range(3)]
+    want = [int8.linear_int8(t, xs, w, ws) for t in inputs]
+    ref, slack = _linear_reference(inputs[1], xs, w, ws, None, None, torch.float16)
+    assert ((want[1].double() - ref).abs() <= slack).all()
+    graphs = []
+    for _ in range(2):
+        x_in = inputs[0].clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = int8.linear_int8(x_in, xs, w, ws)
+        graphs.append((graph, x_in, y))
+    for turn in range(6):
+        for i, (graph, x_in, y) in enumerate(graphs):
+            at = (turn + i) % 3
+            x_in.copy_(inputs[at])
+            graph.replay()
+            assert torch.equal(int8.linear_int8(inputs[at], xs, w, ws), want[at])
+            assert torch.equal(y, want[at])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for turn in range(3):
+        for i, (_, x_in, _) in enumerate(graphs):
+            x_in.copy_(inputs[(turn + i) % 3])
+        torch.cuda.synchronize()
+        for stream, (graph, _, _) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for i, (_, _, y) in enumerate(graphs):
+            assert torch.equal(y, want[(turn + i) % 3])
