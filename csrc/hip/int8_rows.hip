@@ -488,8 +488,12 @@ constexpr long long kMostRows = 1ll << 21;
 // has on their way: 64 do best, 32 where each CU has few rows.  Times with one, two and four chunks per thread, bf16 from
 // memory: 16384 rows of 8192 quantised 120, 87 and 74 us (16 bytes of input a chunk), the norm with a residual 184, 169 and
 // 172, the gate 138, 125 and 122 (32 bytes); 2048 rows of 4096 10.6, 9.9 and 11.0; 16.0, 17.4 and 19.0; 12.3, 12.2 and 13.6.
-// The gate's blocks stay at 512 threads (4096 rows of 16384: 65.0 us, 67.6 with 1024).  Norms of fp32 rows hold three fp32
-// inputs per value: two chunks are what the registers of 1024 threads hold.
+// The gate keeps to two: four, in blocks of 512 threads, gain little where they fill the block (4096 rows of 16384: 62.5 us,
+// 63.3 with two) and lose where they do not (of 8200 36.6 and 33.0, of 12000 53.3 and 48.0; fp32 rows of 8200 69.4 and 55.5).
+// Norms of fp32 rows hold three fp32 inputs per value: two chunks are what the registers of 1024 threads hold.  Of the kernels
+// of four, two spill 4 and 8 registers, for rows of more than 16384 values, which would be read twice otherwise: the gate of
+// fp32 rows is faster all the same (2048 of 20000 92 and 100 us, of 32768 136 and 164), and the norm with a residual of bf16
+// rows and an fp32 weight with few rows (256 of 32768 14.6 and 17.4 us, 2048 of them 125 and 119).
 template <typename T, typename W, int kMode>
 void LaunchRows(RowArgs a, hipStream_t stream) {
   constexpr bool kWide = sizeof(T) == 4 && (kMode == kNorm || kMode == kNormResidual);
@@ -500,8 +504,7 @@ void LaunchRows(RowArgs a, hipStream_t stream) {
   const int bytes = rows >= 4096 ? 64 : 32;
   int per_thread = rows >= 1024 && chunks >= 512 ? bytes / (kInputs * kVec * static_cast<int>(sizeof(T))) : 1;
   per_thread = per_thread < 1 ? 1 : per_thread < most ? per_thread : most;
-  const int most_threads = kMode == kGate && rows >= 1024 ? 512 : 1024;
-  while (per_thread < most && chunks > per_thread * most_threads) per_thread *= 2;
+  while (per_thread < most && chunks > per_thread * 1024) per_thread *= 2;
   const dim3 threads(((chunks + per_thread - 1) / per_thread + 63) / 64 * 64);
   for (; a.first_row < rows; a.first_row += kMostRows) {
     const unsigned count = static_cast<unsigned>(rows - a.first_row < kMostRows ? rows - a.first_row : kMostRows);

@@ -855,3 +855,21 @@ def test_destinations_in_a_graph():
         t.zero_()
         graph.replay()
         assert torch.equal(t, int8.dequantize_int8(q, s, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows", [5, 1030, 4100])
+@pytest.mark.parametrize("width", [4104, 8200, 12000, 16384, 20000])
+def test_gate_of_wide_rows(width, rows, dtype):
+    """Against the formula, in every split of a row: chunks that fill the threads of a block, and that do not."""
+    g = torch.Generator(device="cuda").manual_seed(width)
+    x = (2 * torch.randn(rows, 2 * width, generator=g, device="cuda")).to(dtype)
+    q, scale = int8.silu_mul_int8(x)
+    for at in (0, rows // 2, rows - 3):
+        gate, up = x[at:at + 3].double().chunk(2, dim=-1)
+        p = gate / (1 + torch.exp(-gate)) * up
+        top = p.abs().amax(dim=-1, keepdim=True)
+        assert ((q[at:at + 3].double() - 127 * p / top).abs() <= 0.5 + 127 * 16.1 * F32).all()  # as in test_gate
+        assert ((scale[at:at + 3].double() - top[:, 0] / 127).abs() <= 9.1 * F32 * top[:, 0] / 127).all()
+    few = int8.silu_mul_int8(x[-4:])  # in the split of few rows
+    assert torch.equal(q[-4:], few[0]) and torch.equal(scale[-4:], few[1])
