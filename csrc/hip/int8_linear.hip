@@ -17,10 +17,11 @@
 // SplitAnyKernel, TileAnyKernel  the same, and tiles of 64 x 64, for rows that do not start at multiples of 16 bytes, through
 //              registers.
 // TileKernel   large products: tiles of 64 x 64 to 256 x 256 outputs per block of four waves, operands through LDS stages
-//              filled by DMA.  8192 x 8192 x 8192 to bf16: 371 to 395 us on two cards (2.8 to 3.0 POP/s), 382 to 411 with a
-//              residual.  What bounds it is the card's power: on zeros, where nothing toggles, the same call took 296 us (312
-//              with a residual) on the faster one, and its products alone, fed from registers, 293 us on real values and
-//              259 on zeros.  One wave per SIMD with 128 x 128 outputs reads the fewest bytes from LDS per product and won
+//              filled by DMA.  8192 x 8192 x 8192 to bf16, one call behind another on real values: 385 us (2.9 POP/s), 423
+//              with a residual.  What bounds it is the card's power, so that the time goes with what ran before: 5 calls after
+//              a pause 392 and 424, 20 calls 456 and 491, one alone 447 and 456.  On zeros, where nothing toggles, it took 296
+//              and 312 on a card that took 371 and 382 on values, and its products alone, fed from registers, 293 us on
+//              values and 259 on zeros.  One wave per SIMD with 128 x 128 outputs reads the fewest bytes from LDS per product and won
 //              over two waves with 128 x 64 (408 against 420 us at an earlier stage of tuning); products of 16 x 16 x 64
 //              touch the accumulators half as often per operation as those of 32 x 32 x 32 and won although they issue
 //              twice as often (443 against 476 us, earlier still).
@@ -987,9 +988,11 @@ constexpr Way kAligned[] = {{256, 256, 1, 1, 1.16f, 6.96f, 0.18f, 0.80f, 0.86f},
                             {16, 16, 4, 5, 0.20f, 0.76f, 0.18f, 0.40f, 0.62f},   {16, 16, 2, 10, 0.20f, 0.73f, 0.10f, 0.24f, 0.60f}};
 
 // Few tokens are bound by memory, and what differs is how the rows that are asked for at a time fall on its channels, which
-// the estimates do not know: tiles of 16 weight rows do best where rows are multiples of 8 KB apart (16 x 6144 x 8192: 10.8
-// us, where 32 rows take 13.9), and for a large weight and up to eight tokens one of them does as well as any (1 x 16384 x
-// 8192: 22.9 us against 29.1 with 32 rows).
+// the estimates do not know.  Tiles of 16 weight rows do best where rows are multiples of 8 KB apart: 16 x 6144 x 8192 13.5
+// us, 15.5 with 32 rows; from 17 tokens on that is over (17 x 6144 x 8192: 14.6 with 16 rows, 14.8 with 64).  For up to eight
+// tokens and a large weight one of them stands for all: 1 x 16384 x 8192 23.9 us (26.4 with 64 rows), 8 x 4096 x 16384
+// 18.6 (25.4); with rows 4 KB apart 64 rows would do better (1 x 16384 x 4096 16.1 and not 16.9, 1 x 28672 x 4096 24.0 and
+// not 27.2), and nine tokens, which the estimates place, have them (16.1 and 24.3).
 constexpr long long kStreams = 64ll << 20;
 
 int AlignedWay(const LinearArgs& a) {

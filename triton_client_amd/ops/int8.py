@@ -273,8 +273,8 @@ def rms_norm_int8(x, weight, residual=None, eps=1e-6, out=None, scale=None, sum_
               normalised and returned: what the next block reads is what this one saw
     sum_out   destination of the sum; may be ``x`` or ``residual`` itself
 
-    ``q`` is the integer nearest to ``127 h weight / max|h weight|`` (ties to even, decided exactly): the norm's factor
-    cancels and only enters the scale.  Sums of squares are held in 64 bits."""
+    ``q`` is the integer nearest to ``127 p / max|p|`` (ties to even, decided exactly) for ``p = h weight`` in fp32: the
+    norm's factor cancels and only enters the scale.  Sums of squares are held in 64 bits."""
     if out is None and scale is None and sum_out is None:
         made = (_plain or _load_plain()).rms_norm(x, weight, residual, eps)
         if made is not None:
@@ -370,7 +370,7 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
     residual              ``[..., N]`` in ``dtype``, or None; ``out`` may be the residual itself
 
     Sums are int32 and exact for K up to 131071; scales, bias and residual are applied in fp32 and the result is rounded
-    once.  Operands whose rows start at multiples of 16 bytes (K and the row strides multiples of 16) are read as they are;
+    once.  The product of the two scales is taken first: where it leaves fp32's normal range the result does, too.  Operands whose rows start at multiples of 16 bytes (K and the row strides multiples of 16) are read as they are;
     others are read more slowly or, in a large product, first copied to such rows in a workspace of the call."""
     if out is None:
         code = _output_code(torch.float16 if dtype is None else dtype)
