@@ -13,6 +13,7 @@
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -45,6 +46,13 @@ at::ScalarType Type(long code) { return code == 0 ? at::kFloat : code == 1 ? at:
 
 constexpr long long kMostWidth = 1ll << 29, kMostK = 131071;
 
+// Whether something records this thread's operations: torch.jit.trace, or make_fx, at either of its levels.
+bool Traced() {
+  return at::tracer::impl::is_dispatch_enabled() ||
+         c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+}
+
 // A plain operand: a contiguous tensor on the current CUDA device that needs no gradient and has no tangent, in a call that
 // nothing traces.  `device` is set by the first operand (-1 before it): without a GPU there is no current device to ask for.
 struct Operand {
@@ -56,7 +64,7 @@ struct Operand {
         t->_fw_grad(0).defined())
       return false;
     if (device < 0) {
-      if (at::tracer::impl::is_dispatch_enabled() || c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
+      if (Traced()) return false;
       device = t->device().index();
       return c10::hip::current_device() == device;
     }

@@ -804,7 +804,28 @@ def test_tangents_and_traces_on_the_gpu():
 
     torch.jit.trace(traced, (x,), check_trace=False)
     make_fx(traced)(x)
+    make_fx(traced, pre_dispatch=True)(x)
     assert torch.equal(ops.quantize(x, False)[0], q)
+
+
+def test_plain_calls_under_other_modes():
+    """A mode that watches operators, or a wrapped program, changes nothing."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = _values(3, 32, torch.float16).cuda()
+    q, s = int8.quantize_int8(x)
+    with Watch():
+        got = int8.quantize_int8(x)
+        strided = int8.quantize_int8(x[:, ::2])
+    assert torch.equal(got[0], q) and torch.equal(got[1], s)
+    assert torch.equal(strided[0], int8.quantize_int8(x[:, ::2])[0])
+    compiled = torch.compile(lambda t: int8.dequantize_int8(*int8.quantize_int8(t + 1), dtype=torch.float32) * 2, backend="eager")
+    want = int8.dequantize_int8(*int8.quantize_int8(x + 1), dtype=torch.float32) * 2
+    assert torch.equal(compiled(x), want) and torch.equal(compiled(x), want)
 
 
 def test_destinations_that_a_backward_pass_has_saved():

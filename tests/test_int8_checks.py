@@ -190,6 +190,7 @@ def test_traces_are_refused():
 
     torch.jit.trace(f, (torch.ones(2, 8),), check_trace=False)
     make_fx(f)(torch.ones(2, 8))
-    assert len(seen) == 2 * len(_every_call(torch.ones(2, 8)))
+    make_fx(f, pre_dispatch=True)(torch.ones(2, 8))
+    assert len(seen) == 3 * len(_every_call(torch.ones(2, 8)))
     with pytest.raises(ValueError, match="CUDA"):
         int8.quantize_int8(torch.ones(2, 8))

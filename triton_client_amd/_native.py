@@ -173,7 +173,7 @@ def torch_ops():
 
             _build.build_torch()
             from ._lib import _tca_torch
-        here = f"{torch.__version__} {torch.version.git_version}"
+        here = f"{torch.__version__} {getattr(torch.version, 'git_version', '')}"
         built_for = getattr(_tca_torch, "built_for", "one that it does not name")
         if built_for != here:
             raise ImportError(f"_tca_torch was built for torch {built_for}, this is {here}: "
