@@ -99,7 +99,8 @@ def build_torch(force=False):
     src = CSRC / "capi" / "torch_ops.cc"
     version = (home / "version.py").read_text()
     # as _native.torch_ops() puts it together from the imported torch
-    torch = " ".join("".join(re.findall(rf"^{name} = ['\"](.*)['\"]", version, re.M)) for name in ("__version__", "git_version"))
+    torch = " ".join("".join(re.findall(rf"^{name} = ['\"](.*)['\"]", version, re.M))
+                     for name in ("__version__", "git_version"))
     built_for = LIBDIR / "_tca_torch.torch"
     if (force or _stale(out, [src, CSRC / "hip" / "kernels.h", home / "version.py"])
             or not built_for.exists() or built_for.read_text() != torch):

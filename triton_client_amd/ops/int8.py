@@ -372,7 +372,8 @@ def linear_int8(x, x_scale, weight, weight_scale, bias=None, residual=None, dtyp
     Sums are int32 and exact for K up to 131071; scales, bias and residual are applied in fp32 and the result is rounded
     once.  The product of the two scales is taken first, in fp32: below 1.2e-38 it has fewer digits, and the result with it;
     beyond 3.4e38 it is infinite.  Operands whose rows start at multiples of 16 bytes (K and the row strides multiples of
-    16) are read as they are; others are read more slowly or, in a large product, first copied to such rows in a workspace of the call."""
+    16) are read as they are; others are read more slowly or, in a large product, first copied to such rows in a workspace
+    of the call."""
     if out is None:
         code = _output_code(torch.float16 if dtype is None else dtype)
         made = (_plain or _load_plain()).linear(x, x_scale, weight, weight_scale, bias, residual, code)
